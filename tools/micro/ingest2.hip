@@ -4,7 +4,7 @@
 //   mode 1: global_load_dwordx4 into registers only (two register sets in flight), nothing written to LDS
 //   mode 2: global_load_dwordx4 into registers, then ds_write_b128 into a 2-deep LDS ring + barrier per K-step
 // for the tile shapes a nav-step GEMM could use.  Prints us per launch and B/clk/CU; answers "what bounds the K loop".
-// build: hipcc -O3 --offload-arch=gfx950 tools/micro/ingest2.hip -o gpurun_out/ingest2
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/micro/ingest2.hip -o gpurun_out/ingest2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
