@@ -7,11 +7,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('DSRG_HIP_LIB') or os.path.join(_HERE, 'csrc', 'libdsrg_hip.so')
 
 F32, BF16 = 0, 1
+I8, E4M3 = 2, 3          # storage of a key / value cache only
 ACT_NONE, ACT_GELU, ACT_RELU, ACT_TANH = 0, 1, 2, 3
 MASK_NONE, MASK_NEG10000, MASK_NEGINF, MASK_PLUS1 = 0, 1, 2, 3
 IDX_I32, IDX_I64, IDX_F32 = 0, 1, 2
 MAX_GROUPS = 8
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 
 class HeadTailProblem(C.Structure):
@@ -73,6 +74,12 @@ class LnProblem(C.Structure):
                 ('M', C.c_int32), ('ldx', C.c_int32), ('ldr', C.c_int32), ('ldo', C.c_int32),
                 ('o_seg', C.c_int32), ('o_seg_ld', C.c_int32), ('aux0', C.c_void_p), ('aux1', C.c_void_p),
                 ('aux_seg', C.c_int32), ('aux_ld0', C.c_int32), ('aux_ld1', C.c_int32), ('reserved_', C.c_int32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [('k_pool', C.c_void_p), ('v_pool', C.c_void_p), ('k_scale', C.c_void_p), ('v_scale', C.c_void_p),
+                ('n_pages', C.c_int32), ('page_size', C.c_int32), ('n_kv_heads', C.c_int32), ('head_dim', C.c_int32),
+                ('dtype', C.c_int32), ('reserved_', C.c_int32)]
 
 
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -139,6 +146,11 @@ SIGNATURES = {
     'dsrg_graph_update_embeds': (C.c_int, [C.POINTER(GraphState), _P, _P, _P, _P, _I, _P, _L, _I, _P, _I, _I, _I, _P]),
     'dsrg_graph_nav_inputs': (C.c_int, [C.POINTER(GraphState), C.POINTER(GraphNavOut), _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     'dsrg_action_tail_fwd': (C.c_int, [_P, _I, _P, _L, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    'dsrg_sample_rows': (C.c_int, [_P, _L, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _I, _I, _P]),
+    'dsrg_kv_append': (C.c_int, [C.POINTER(KvCache), _P, _L, _I, _P, _L, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P]),
+    'dsrg_kv_read': (C.c_int, [C.POINTER(KvCache), _P, _L, _I, _P, _L, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P]),
+    'dsrg_attention_paged_workspace': (C.c_int64, [C.POINTER(KvCache), _I, _I, _I, _I, _I]),
+    'dsrg_attention_paged': (C.c_int, [C.POINTER(KvCache), _P, _L, _I, _P, _L, _I, _P, _P, _I, _I, _P, _I, _I, _I, _F, _I, _I, _P, _L, _I, _P]),
     'dsrg_ce_rows_fwd': (C.c_int, [_P, _I, _P, _L, _P, _P, _I, _I, _P]),
     'dsrg_ce_rows_bwd': (C.c_int, [_P, _I, _P, _L, _P, _P, _P, _I, _I, _I, _I, _P]),
     'dsrg_igl_blend_fwd': (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),

@@ -1,0 +1,709 @@
+// Paged key / value cache (gfx950): write (with quantisation), read back, and attention of a few new tokens over it.
+//
+// Layout (include/dsrg_hip.h, dsrg_kv_cache_t).  A page holds S tokens of every head; inside (page, head) the keys of 16
+// tokens and the values of 32 tokens lie in the order in which an MFMA operand fragment wants them, so that a wave's load of
+// one fragment is one contiguous run of 64 x 16 bytes (8-bit codes: 64 x 8) and needs neither LDS nor a transposition:
+//   K  [S/16][D/8][16 tokens][8 dims]                    A operand of S^T = K . Q^T: lane (g, r) = token r, dims 32 s + 8 g ..
+//   V  [S/32][D/16][4 g][16 dims][2 m][4 i]              A operand of O^T = V^T . P^T: lane (g, d) = dim d, tokens 16 m + 4 g + i
+// The second one follows from the first product's result: lane (g, c) holds the scores of query c against tokens 4 g + i of each
+// 16-token tile, so two tiles' registers ARE the B operand of the second product if the contraction index runs over the tokens
+// in the order (m, i) per g - and V is stored in that order.  fp32 (v_mfma_f32_16x16x4_f32, one token or dim per step and lane
+// group): 4-element chunks, K [S/16][D/4][16][4], V [S/16][D/16][4 g][16][4 i].
+#include "common.h"
+#include <math.h>
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint8_t u8;
+
+namespace {
+
+constexpr float KV_TINY = 1.17549435e-38f;      // smallest scale (2^-126): a row of zeros has it
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+template <int KV> struct KvT;
+template <> struct KvT<DSRG_F32> { typedef float type; static constexpr int SZ = 4, E = 4; };
+template <> struct KvT<DSRG_BF16> { typedef bf16_t type; static constexpr int SZ = 2, E = 8; };
+template <> struct KvT<DSRG_I8> { typedef u8 type; static constexpr int SZ = 1, E = 8; };
+template <> struct KvT<DSRG_E4M3> { typedef u8 type; static constexpr int SZ = 1, E = 8; };
+
+struct Pool {
+  void* k; void* v; float* ks; float* vs;
+  int P, S, lgS, H;
+};
+
+// element offset of dim d of token r (within a page's head) in K / V
+template <int KV, int D> __device__ __forceinline__ int k_off(int r, int d) {
+  constexpr int E = KvT<KV>::E;
+  return (r >> 4) * 16 * D + ((d / E) * 16 + (r & 15)) * E + d % E;
+}
+template <int KV, int D> __device__ __forceinline__ int v_off(int r, int d) {
+  if (KvT<KV>::E == 4) return (r >> 4) * 16 * D + (((d >> 4) * 4 + ((r & 15) >> 2)) * 16 + (d & 15)) * 4 + (r & 3);
+  return (r >> 5) * 32 * D + (((d >> 4) * 4 + ((r & 15) >> 2)) * 16 + (d & 15)) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
+}
+
+// ---- 8-bit codes ---------------------------------------------------------------------------------------------------------
+// scale = max(amax * (1 / most), 2^-126), code = round-to-nearest-even(x / scale), clamped (amax / scale can round past `most`).
+// A row with a NaN or an infinity has no scale: it gets NaN, so that every value read back from it is NaN, not a wrong number.
+template <int KV> __device__ __forceinline__ float kv_scale(float amax, bool finite) {
+  const float s = fmaxf(amax * (KV == DSRG_I8 ? (float)(1.0 / 127.0) : (float)(1.0 / 448.0)), KV_TINY);
+  return finite ? s : __builtin_nanf("");
+}
+template <int KV> __device__ __forceinline__ unsigned kv_code(float x, float scale) {
+  constexpr float MOST = KV == DSRG_I8 ? 127.f : 448.f;
+  const float y = fminf(fmaxf(x / scale, -MOST), MOST);          // (NaN: fmaxf gives -MOST, a valid code)
+  if (KV == DSRG_I8) return (unsigned)(int)rintf(y) & 0xffu;
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xffu;
+}
+template <int KV> __device__ __forceinline__ float kv_value(unsigned code) {
+  if (KV == DSRG_I8) return (float)(int)(int8_t)code;
+  return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+}
+
+template <typename T> __device__ __forceinline__ void ld8(const T* p, float (&x)[8]) {      // 16-byte aligned
+  const float4 a = ld4(p), b = ld4(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// maximum over the D / 8 lanes (8 or 16, aligned) that hold one row
+template <int D> __device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_mov_f32<0xB1>(v));
+  v = fmaxf(v, dpp_mov_f32<0x4E>(v));
+  v = fmaxf(v, dpp_mov_f32<0x141>(v));
+  if (D == 128) v = fmaxf(v, dpp_mov_f32<0x140>(v));
+  return v;
+}
+
+// ---- write ---------------------------------------------------------------------------------------------------------------
+struct AppendArgs {
+  Pool c;
+  const void *k, *v;
+  long long k_bs, v_bs;
+  int k_rs, v_rs;
+  const int32_t *table, *start, *count;
+  int table_ld, width, B, T;
+};
+
+// D / 8 lanes per (sequence, token, head) row, 8 dims each, K and V of the row by the same lanes.
+template <int KV, int D, typename TI>
+__global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
+  typedef typename KvT<KV>::type TS;
+  constexpr int LPR = D / 8;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int d0 = (threadIdx.x % LPR) * 8, H = a.c.H;
+  if (row >= (long long)a.B * a.T * H) return;          // whole rows leave together: the DPP steps below stay inside a row's lanes
+  const int h = (int)(row % H);
+  const long long bt = row / H;
+  const int b = (int)(bt / a.T), t = (int)(bt % a.T);
+  if (a.count && t >= a.count[b]) return;
+  const long long pos = (long long)a.start[b] + t;
+  if (pos < 0 || pos >= (long long)a.width * a.c.S) return;
+  const int page = a.table[(long long)b * a.table_ld + (pos >> a.c.lgS)], r = (int)pos & (a.c.S - 1);
+  if (page < 0 || page >= a.c.P) return;
+  const long long ph = (long long)page * H + h;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const TI* src = (const TI*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (long long)t * (which ? a.v_rs : a.k_rs) + h * D + d0;
+    float x[8];
+    ld8(src, x);
+    TS* dst = (TS*)(which ? a.c.v : a.c.k) + ph * a.c.S * D;
+    TS w[8];
+    if (KvT<KV>::SZ == 1) {
+      float m = 0.f;
+      bool fin = true;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { m = fmaxf(m, fabsf(x[j])); fin = fin && fabsf(x[j]) <= 3.4028235e38f; }
+      m = row_max<D>(fin ? m : INFINITY);
+      const float s = kv_scale<KV>(m, m <= 3.4028235e38f);
+      if (d0 == 0) (which ? a.c.vs : a.c.ks)[ph * a.c.S + r] = s;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = (TS)kv_code<KV>(x[j], s);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) Elem<typename std::conditional<KV == DSRG_F32, float, bf16_t>::type>::st((typename std::conditional<KV == DSRG_F32, float, bf16_t>::type*)&w[j], x[j]);
+    }
+    if (which == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; j += KvT<KV>::E) __builtin_memcpy(__builtin_assume_aligned(dst + k_off<KV, D>(r, d0 + j), KvT<KV>::E * KvT<KV>::SZ), &w[j], KvT<KV>::E * KvT<KV>::SZ);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dst[v_off<KV, D>(r, d0 + j)] = w[j];
+    }
+  }
+}
+
+// ---- read back -----------------------------------------------------------------------------------------------------------
+struct ReadArgs {
+  Pool c;
+  void *k, *v;
+  long long k_bs, v_bs;
+  int k_rs, v_rs;
+  const int32_t *table, *start, *count;
+  int table_ld, width, B, N;
+};
+
+// Same lanes as the write; a row past the sequence's count (or on no page) is zero.
+template <int KV, int D, typename TO>
+__global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
+  typedef typename KvT<KV>::type TS;
+  constexpr int LPR = D / 8;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int d0 = (threadIdx.x % LPR) * 8, H = a.c.H;
+  if (row >= (long long)a.B * a.N * H) return;
+  const int h = (int)(row % H);
+  const long long bt = row / H;
+  const int b = (int)(bt / a.N), t = (int)(bt % a.N);
+  const long long pos = (long long)(a.start ? a.start[b] : 0) + t;
+  int page = -1;
+  if (t < a.count[b] && pos >= 0 && pos < (long long)a.width * a.c.S) page = a.table[(long long)b * a.table_ld + (pos >> a.c.lgS)];
+  const bool live = page >= 0 && page < a.c.P;
+  const int r = (int)pos & (a.c.S - 1);
+  const long long ph = (long long)page * H + h;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (live) {
+      const TS* src = (const TS*)(which ? a.c.v : a.c.k) + ph * a.c.S * D;
+      const float s = KvT<KV>::SZ == 1 ? (which ? a.c.vs : a.c.ks)[ph * a.c.S + r] : 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const TS e = src[which ? v_off<KV, D>(r, d0 + j) : k_off<KV, D>(r, d0 + j)];
+        if constexpr (KvT<KV>::SZ == 1) x[j] = kv_value<KV>(e) * s;
+        else x[j] = Elem<TS>::ld(&e);
+      }
+    }
+    TO* dst = (TO*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (long long)t * (which ? a.v_rs : a.k_rs) + h * D + d0;
+    st4(dst, make_float4(x[0], x[1], x[2], x[3]));
+    st4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+  }
+}
+
+// ---- attention over the cache ----------------------------------------------------------------------------------------------
+//   o[b, i, h] = sum_t softmax_t(scale * q[b, i, h] . k[t, h / G]) v[t, h / G]     over the tokens t that row i sees
+// The Nq * G query rows that share a key / value head are the columns of S^T = K . Q^T (16 per MFMA tile; one new token with
+// G = 1 fills one of them, which costs nothing: the loop waits for memory).  A wave takes 32 tokens a time: two score tiles,
+// the running maximum and sum per column (maximum of a lane's 8 scores, then over the four lane groups), P straight from the
+// score registers into the B operand of O^T += V^T . P^T.  Waves share nothing until the end: they take blocks in turn and are
+// joined in LDS.  Few sequences: the tokens are also split over workgroups, whose (maximum, sum, O) are joined by a second kernel.
+struct PagedArgs {
+  Pool c;
+  const void* q; void* o; float* lse;
+  long long q_bs, o_bs;
+  int q_rs, o_rs;
+  const int32_t *table, *lens;
+  int table_ld, width, B, nh, G, Nq, NC;       // NC = Nq * G columns per (sequence, key / value head)
+  int causal, window, nsplit, bps;             // bps: 32-token blocks per split
+  float sl2;                                   // scale * log2(e)
+  float* ws_o; float2* ws_ml;                  // [B, H, NC, nsplit, D], [B, H, NC, nsplit]
+};
+
+// maximum / sum over the four lanes (one per 16-lane row) of a column
+__device__ __forceinline__ float col_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+__device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
+  bf16x8 r;
+  if (kv == DSRG_E4M3) {
+    bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.x, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.x, 1.0f, true);
+    bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.y, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.y, 1.0f, true);
+    r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1]; r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r[j] = (__bf16)(float)((int)(u.x << (24 - 8 * j)) >> 24);
+      r[4 + j] = (__bf16)(float)((int)(u.y << (24 - 8 * j)) >> 24);
+    }
+  }
+  return r;
+}
+
+// MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
+template <int KV, int D, int CT, int NW, bool MIX>
+__global__ __launch_bounds__(NW * 64) void attention_paged_kernel(const PagedArgs a) {
+  typedef typename KvT<KV>::type TS;
+  typedef typename std::conditional<KV == DSRG_F32, float, bf16_t>::type TQ;
+  constexpr bool F = KV == DSRG_F32, Q8 = KvT<KV>::SZ == 1;
+  constexpr int KS = F ? D / 16 : D / 32;        // 16-byte (8-byte) key chunks of a lane per 16-token tile
+  constexpr int DT = D / 16;
+  constexpr int OLD = D + 4;
+  __shared__ float so[NW][16][OLD];
+  __shared__ float sm[NW][16], sl[NW][16];
+  const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sp = blockIdx.x, H = a.c.H, kh = blockIdx.y % H, cg = blockIdx.y / H, b = blockIdx.z;
+  const int cap = a.width * a.c.S;
+  const int len = min(max(a.lens[b], 0), cap);
+  const int lo_all = a.window ? max(0, len - a.Nq - a.window + 1) : 0;       // first token any row sees
+  const int blk0 = lo_all >> 5, blk_end = (len + 31) >> 5;
+  const int bbeg = blk0 + sp * a.bps, bend = min(bbeg + a.bps, blk_end);
+  if (a.nsplit > 1 && bbeg >= bend) return;                                  // (the joining kernel skips the split as well)
+
+  // queries and what each column sees: [lo, hi)
+  int hi[CT], lo[CT];
+  using QF = typename std::conditional<F, float4, bf16x8>::type;
+  QF qf[CT][KS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int n = (cg * CT + ct) * 16 + c16;
+    const bool live = n < a.NC;
+    const int i = live ? n / a.G : 0, h = kh * a.G + (live ? n - i * a.G : 0);
+    hi[ct] = !MIX ? len : !live ? 0 : max(0, len - a.Nq + i + 1);
+    lo[ct] = !MIX ? lo_all : a.window ? max(0, hi[ct] - a.window) : 0;
+    const TQ* qp = (const TQ*)a.q + b * a.q_bs + (long long)i * a.q_rs + (long long)h * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (F) qf[ct][s] = live ? *reinterpret_cast<const float4*>(qp + 16 * s + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
+      else {
+        uint4 u = live ? *reinterpret_cast<const uint4*>(qp + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+        qf[ct][s] = __builtin_bit_cast(bf16x8, u);
+      }
+    }
+  }
+  // blocks in [full_lo, full_hi) are seen whole by every live column
+  const int full_hi = (MIX ? max(0, len - a.Nq + 1) : len) >> 5, full_lo = a.window ? (max(0, len - a.window) + 31) >> 5 : 0;
+
+  f32x4 o[CT][DT];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY; l[ct] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* trow = a.table + (long long)b * a.table_ld;
+  const int lgB = a.c.lgS - 5, bmask = (1 << lgB) - 1;
+  for (int blk = bbeg + w; blk < bend; blk += NW) {
+    const int page = __builtin_amdgcn_readfirstlane(trow[blk >> lgB]);
+    if (page < 0 || page >= a.c.P) continue;                 // no such page: its tokens are masked
+    const long long ph = (long long)page * H + kh;
+    const long long e0 = (ph * a.c.S + (blk & bmask) * 32) * D;
+    const TS* kb = (const TS*)a.c.k + e0;
+    const TS* vb = (const TS*)a.c.v + e0;
+    using RF = typename std::conditional<F, float4, typename std::conditional<Q8, uint2, uint4>::type>::type;
+    constexpr int E = KvT<KV>::E;
+    RF kr[2][KS], vr[F ? 2 * DT : DT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const RF*>(kb + t * 16 * D + (s * 64 + lane) * E);
+    float4 ksc[2], vsc[2];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const long long so_ = ph * a.c.S + (blk & bmask) * 32 + 16 * t + 4 * g;
+        ksc[t] = *reinterpret_cast<const float4*>(a.c.ks + so_);
+        vsc[t] = *reinterpret_cast<const float4*>(a.c.vs + so_);
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt) vr[dt] = *reinterpret_cast<const RF*>(vb + (dt * 64 + lane) * E);
+    const bool full = blk >= full_lo && blk < full_hi;
+
+    f32x4 s_[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s_[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (F) {
+          const float kf[4] = {kr[t][s].x, kr[t][s].y, kr[t][s].z, kr[t][s].w};
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const float qq[4] = {qf[ct][s].x, qf[ct][s].y, qf[ct][s].z, qf[ct][s].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s_[ct][t], 0, 0, 0);
+          }
+        } else {
+          bf16x8 kf;
+          if constexpr (Q8) kf = codes_to_bf16(kr[t][s], KV);
+          else kf = __builtin_bit_cast(bf16x8, kr[t][s]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][s], s_[ct][t], 0, 0, 0);
+        }
+      }
+
+    const int key0 = blk * 32 + 4 * g;
+    float p[CT][8];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s_[ct][t][i] * a.sl2;
+          if constexpr (Q8) x *= (&ksc[t].x)[i];
+          if (!full) { const int key = key0 + 16 * t + i; x = key < hi[ct] && key >= lo[ct] ? x : -INFINITY; }
+          p[ct][4 * t + i] = x;
+          mx = fmaxf(mx, x);
+        }
+      const float mn = fmaxf(m[ct], col_max(mx));
+      if (__any(mn > m[ct])) {
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mn);
+        l[ct] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[ct][dt] *= f;
+        m[ct] = mn;
+      }
+      const float mb = m[ct] == -INFINITY ? 0.f : m[ct];
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { p[ct][j] = __builtin_amdgcn_exp2f(p[ct][j] - mb); sum += p[ct][j]; }
+      l[ct] += sum;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[ct][4 * t + i] = (full || p[ct][4 * t + i] != 0.f) ? p[ct][4 * t + i] * (&vsc[t].x)[i] : 0.f;
+      }
+    }
+
+    // Tokens of a block that not every column sees may hold anything, and 0 * NaN is NaN: what no column sees is zeroed here,
+    // what only some columns see is looked at below.
+    if (!full) {
+      const int h_all = len, l_all = lo_all;
+#pragma unroll
+      for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt)
+#pragma unroll
+        for (int j = 0; j < (F ? 4 : 8); ++j) {
+          const int key = key0 + (F ? 16 * (dt / DT) + j : 16 * (j >> 2) + (j & 3));
+          const bool in = key < h_all && key >= l_all;
+          if constexpr (F) (&vr[dt].x)[j] = in ? (&vr[dt].x)[j] : 0.f;
+          else if constexpr (Q8) { unsigned& u = j < 4 ? vr[dt].x : vr[dt].y; u = in ? u : u & ~(0xffu << (8 * (j & 3))); }
+          else { unsigned& u = (&vr[dt].x)[j >> 1]; u = in ? u : u & (j & 1 ? 0x0000ffffu : 0xffff0000u); }
+        }
+    }
+    bool each = false;
+    if constexpr (MIX && !Q8) {
+      // (8-bit codes of a written row are finite, and the scale above is only taken where the token is seen)
+      if (!full) {
+        bool bad = false;
+#pragma unroll
+        for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (F) bad = bad || !(fabsf((&vr[dt].x)[j]) <= 3.4028235e38f);
+            else { const unsigned u = (&vr[dt].x)[j]; bad = bad || (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; }
+          }
+        each = __any(bad);
+      }
+      if (each) {                       // a value that is not finite in a block that only some columns see: column by column
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll 1
+          for (int col = 0; col < 16; ++col) {
+            const int ch = __shfl(hi[ct], col), cl = __shfl(lo[ct], col);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              f32x4 r = o[ct][dt];
+              if constexpr (F) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 16 * t + i;
+                    r = __builtin_amdgcn_mfma_f32_16x16x4f32(key >= cl && key < ch ? (&vr[t * DT + dt].x)[i] : 0.f, p[ct][4 * t + i], r, 0, 0, 0);
+                  }
+              } else {
+                bf16x8 pf, vf = __builtin_bit_cast(bf16x8, vr[dt]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const int key = key0 + 16 * (j >> 2) + (j & 3);
+                  pf[j] = (__bf16)p[ct][j];
+                  vf[j] = key >= cl && key < ch ? vf[j] : (__bf16)0.f;
+                }
+                r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, r, 0, 0, 0);
+              }
+              if (c16 == col) o[ct][dt] = r;
+            }
+          }
+      }
+    }
+    if (!each)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if constexpr (F) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32((&vr[t * DT + dt].x)[i], p[ct][4 * t + i], o[ct][dt], 0, 0, 0);
+      } else {
+        bf16x8 pf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[j] = (__bf16)p[ct][j];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          bf16x8 vf;
+          if constexpr (Q8) vf = codes_to_bf16(vr[dt], KV);
+          else vf = __builtin_bit_cast(bf16x8, vr[dt]);
+          o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[ct][dt], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // join the waves, one 16-column tile at a time
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int n0 = (cg * CT + ct) * 16, nv = min(16, a.NC - n0);
+    if (ct) __syncthreads();
+    const float ls = col_sum(l[ct]);
+    if (c16 < nv) {
+      if (g == 0) { sm[w][c16] = m[ct]; sl[w][c16] = ls; }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(&so[w][c16][dt * 16 + 4 * g]) = o[ct][dt];
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < nv * (D / 4); idx += NW * 64) {
+      const int c = idx / (D / 4), d = (idx % (D / 4)) * 4, n = n0 + c;
+      float M = -INFINITY;
+#pragma unroll
+      for (int ww = 0; ww < NW; ++ww) M = fmaxf(M, sm[ww][c]);
+      float L = 0.f;
+      f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ww = 0; ww < NW; ++ww) {
+        const float f = sm[ww][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[ww][c] - M);
+        if (f != 0.f) {
+          L += f * sl[ww][c];
+          O += f * *reinterpret_cast<const f32x4*>(&so[ww][c][d]);
+        }
+      }
+      if (a.nsplit == 1) {
+        const int i = n / a.G, h = kh * a.G + n - i * a.G;
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);       // (a NaN sum stays one)
+        st4((TQ*)a.o + b * a.o_bs + (long long)i * a.o_rs + (long long)h * D + d, make_float4(O[0] * inv, O[1] * inv, O[2] * inv, O[3] * inv));
+        if (a.lse && d == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = M == -INFINITY ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+      } else {
+        const long long row = ((long long)b * H + kh) * a.NC + n;
+        *reinterpret_cast<f32x4*>(a.ws_o + (row * a.nsplit + sp) * D + d) = O;
+        if (d == 0) a.ws_ml[row * a.nsplit + sp] = make_float2(M, L);
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one wave per row, D / 64 dims a lane.
+template <int D, typename TQ>
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedArgs a) {
+  const int lane = threadIdx.x & 63, H = a.c.H;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (long long)a.B * H * a.NC) return;
+  const int n = (int)(row % a.NC), kh = (int)(row / a.NC % H), b = (int)(row / a.NC / H);
+  const int len = min(max(a.lens[b], 0), a.width * a.c.S);
+  const int lo_all = a.window ? max(0, len - a.Nq - a.window + 1) : 0;
+  const int nb = ((len + 31) >> 5) - (lo_all >> 5);
+  const int ns = min(a.nsplit, (nb + a.bps - 1) / a.bps);
+  const float2* ml = a.ws_ml + row * a.nsplit;
+  float M = -INFINITY;
+  for (int s = lane; s < ns; s += 64) M = fmaxf(M, ml[s].x);
+  M = wave_max(M);
+  float L = 0.f, O[D / 64];
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) O[j] = 0.f;
+  if (M != -INFINITY)
+    for (int s = 0; s < ns; ++s) {
+      const float2 v = ml[s];
+      const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
+      if (f != 0.f) {
+        L += f * v.y;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) O[j] += f * a.ws_o[(row * a.nsplit + s) * D + lane + 64 * j];
+      }
+    }
+  const int i = n / a.G, h = kh * a.G + n - i * a.G;
+  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+  TQ* op = (TQ*)a.o + b * a.o_bs + (long long)i * a.o_rs + (long long)h * D;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) Elem<TQ>::st(op + lane + 64 * j, O[j] * inv);
+  if (a.lse && lane == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = M == -INFINITY ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+int check_cache(const dsrg_kv_cache_t* c, const char* who, Pool& p) {
+  DSRG_CHECK(c && c->k_pool && c->v_pool, "%s: cache pools are NULL", who);
+  DSRG_CHECK(c->dtype == DSRG_F32 || c->dtype == DSRG_BF16 || c->dtype == DSRG_I8 || c->dtype == DSRG_E4M3, "%s: unknown cache dtype %d", who, c->dtype);
+  DSRG_CHECK(c->head_dim == 64 || c->head_dim == 128, "%s: head dim %d is not built (64, 128)", who, c->head_dim);
+  DSRG_CHECK(c->page_size >= 32 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0, "%s: page size %d must be a power of two from 32 on", who, c->page_size);
+  DSRG_CHECK(c->n_pages >= 1 && c->n_kv_heads >= 1, "%s: a cache needs pages and heads (%d, %d)", who, c->n_pages, c->n_kv_heads);
+  const bool q8 = c->dtype == DSRG_I8 || c->dtype == DSRG_E4M3;
+  DSRG_CHECK(q8 == (c->k_scale != nullptr) && q8 == (c->v_scale != nullptr), "%s: 8-bit caches need both scale tables, the others none", who);
+  DSRG_CHECK(((uintptr_t)c->k_pool | (uintptr_t)c->v_pool | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 16 == 0, "%s: cache buffers must be 16-byte aligned", who);
+  int lg = 5;
+  while ((1 << lg) < c->page_size) ++lg;
+  p = Pool{c->k_pool, c->v_pool, c->k_scale, c->v_scale, c->n_pages, c->page_size, lg, c->n_kv_heads};
+  return DSRG_OK;
+}
+int check_table(const char* who, const int32_t* table, int ld, int width, int S, int B) {
+  DSRG_CHECK(table && width >= 1 && (ld >= width || B <= 1) && (long long)width * S <= 0x7fffff00ll, "%s: bad page table (width %d, stride %d)", who, width, ld);
+  return DSRG_OK;
+}
+bool rows16(const void* p, long long bs, long long rs, int size) { return (uintptr_t)p % 16 == 0 && bs * size % 16 == 0 && rs * size % 16 == 0; }
+
+struct Split { int nsplit, bps; };
+// Workgroups that the chip should get (256 CUs), and the fewest 32-token blocks that a workgroup should have.
+Split plan_split(int B, int H, int cgs, long long max_tokens) {
+  const long long blocks = (max_tokens + 31) / 32, have = (long long)B * H * cgs;
+  long long ns = (1024 + have - 1) / have;
+  if (ns > (blocks + 7) / 8) ns = (blocks + 7) / 8;
+  if (ns < 1) ns = 1;
+  if (ns > 512) ns = 512;
+  long long bps = (blocks + ns - 1) / ns;
+  if (bps < 1) bps = 1;
+  ns = (blocks + bps - 1) / bps;
+  return Split{(int)(ns < 1 ? 1 : ns), (int)bps};
+}
+long long seen_tokens(int width, int S, int Nq, int window) {
+  const long long cap = (long long)width * S;
+  if (!window) return cap;
+  const long long w = (long long)window + Nq - 1 + 31;       // the first block may start up to 31 tokens early
+  return w < cap ? w : cap;
+}
+int col_tiles(int NC) { return NC > 16 ? 2 : 1; }
+
+}  // namespace
+
+#define KV_SWITCH(DT, ...)                                               \
+  switch (DT) {                                                          \
+    case DSRG_F32: { constexpr int KV = DSRG_F32; __VA_ARGS__; } break;  \
+    case DSRG_BF16: { constexpr int KV = DSRG_BF16; __VA_ARGS__; } break;\
+    case DSRG_I8: { constexpr int KV = DSRG_I8; __VA_ARGS__; } break;    \
+    default: { constexpr int KV = DSRG_E4M3; __VA_ARGS__; } break;       \
+  }
+#define D_SWITCH(HD, ...)                                \
+  if ((HD) == 64) { constexpr int D = 64; __VA_ARGS__; } \
+  else { constexpr int D = 128; __VA_ARGS__; }
+
+static int kv_types_ok(const char* who, int kv, int io) {
+  DSRG_CHECK(io == DSRG_F32 || io == DSRG_BF16, "%s: unsupported dtype %d", who, io);
+  DSRG_CHECK(kv == DSRG_I8 || kv == DSRG_E4M3 || kv == io, "%s: rows of dtype %d for a cache of dtype %d", who, io, kv);
+  return DSRG_OK;
+}
+
+extern "C" int dsrg_kv_append(const dsrg_kv_cache_t* cache, const void* k, int64_t k_bs, int k_rs, const void* v, int64_t v_bs, int v_rs, int dtype,
+                              const int32_t* table, int table_ld, int width, const int32_t* start, const int32_t* count, int B, int T, void* stream) {
+  AppendArgs a;
+  int rc = check_cache(cache, "dsrg_kv_append", a.c);
+  if (rc) return rc;
+  if ((rc = kv_types_ok("dsrg_kv_append", cache->dtype, dtype))) return rc;
+  if (B == 0 || T == 0) return DSRG_OK;
+  DSRG_CHECK(k && v && start && B > 0 && T > 0, "dsrg_kv_append: bad arguments");
+  if ((rc = check_table("dsrg_kv_append", table, table_ld, width, a.c.S, B))) return rc;
+  const int size = dtype == DSRG_F32 ? 4 : 2;
+  DSRG_CHECK(rows16(k, k_bs, k_rs, size) && rows16(v, v_bs, v_rs, size), "dsrg_kv_append: rows must be 16-byte aligned");
+  a.k = k; a.v = v; a.k_bs = k_bs; a.v_bs = v_bs; a.k_rs = k_rs; a.v_rs = v_rs;
+  a.table = table; a.start = start; a.count = count; a.table_ld = table_ld; a.width = width; a.B = B; a.T = T;
+  const long long threads = (long long)B * T * a.c.H * (cache->head_dim / 8), blocks = (threads + 255) / 256;
+  DSRG_CHECK(blocks < (1ll << 31), "dsrg_kv_append: %lld rows in one call", (long long)B * T);
+  const dim3 grid((unsigned)blocks), block(256);
+  KV_SWITCH(cache->dtype, D_SWITCH(cache->head_dim, {
+    if constexpr (KV == DSRG_F32) hipLaunchKernelGGL((kv_append_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
+    else if constexpr (KV == DSRG_BF16) hipLaunchKernelGGL((kv_append_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+    else if (dtype == DSRG_F32) hipLaunchKernelGGL((kv_append_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((kv_append_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+  }))
+  DSRG_LAUNCH_CHECK("dsrg_kv_append");
+  return DSRG_OK;
+}
+
+extern "C" int dsrg_kv_read(const dsrg_kv_cache_t* cache, void* k, int64_t k_bs, int k_rs, void* v, int64_t v_bs, int v_rs, int dtype,
+                            const int32_t* table, int table_ld, int width, const int32_t* start, const int32_t* count, int B, int N, void* stream) {
+  ReadArgs a;
+  int rc = check_cache(cache, "dsrg_kv_read", a.c);
+  if (rc) return rc;
+  if ((rc = kv_types_ok("dsrg_kv_read", cache->dtype, dtype))) return rc;
+  if (B == 0 || N == 0) return DSRG_OK;
+  DSRG_CHECK(k && v && count && B > 0 && N > 0, "dsrg_kv_read: bad arguments");
+  if ((rc = check_table("dsrg_kv_read", table, table_ld, width, a.c.S, B))) return rc;
+  const int size = dtype == DSRG_F32 ? 4 : 2;
+  DSRG_CHECK(rows16(k, k_bs, k_rs, size) && rows16(v, v_bs, v_rs, size), "dsrg_kv_read: rows must be 16-byte aligned");
+  a.k = k; a.v = v; a.k_bs = k_bs; a.v_bs = v_bs; a.k_rs = k_rs; a.v_rs = v_rs;
+  a.table = table; a.start = start; a.count = count; a.table_ld = table_ld; a.width = width; a.B = B; a.N = N;
+  const long long threads = (long long)B * N * a.c.H * (cache->head_dim / 8), blocks = (threads + 255) / 256;
+  DSRG_CHECK(blocks < (1ll << 31), "dsrg_kv_read: %lld rows in one call", (long long)B * N);
+  const dim3 grid((unsigned)blocks), block(256);
+  KV_SWITCH(cache->dtype, D_SWITCH(cache->head_dim, {
+    if constexpr (KV == DSRG_F32) hipLaunchKernelGGL((kv_read_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
+    else if constexpr (KV == DSRG_BF16) hipLaunchKernelGGL((kv_read_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+    else if (dtype == DSRG_F32) hipLaunchKernelGGL((kv_read_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((kv_read_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+  }))
+  DSRG_LAUNCH_CHECK("dsrg_kv_read");
+  return DSRG_OK;
+}
+
+extern "C" int64_t dsrg_attention_paged_workspace(const dsrg_kv_cache_t* cache, int width, int B, int nh, int Nq, int window) {
+  Pool p;
+  const int rc = check_cache(cache, "dsrg_attention_paged_workspace", p);
+  if (rc) return rc;
+  DSRG_CHECK(width >= 1 && B >= 0 && nh >= 1 && nh % p.H == 0 && Nq >= 0 && window >= 0 && (long long)width * p.S <= 0x7fffff00ll, "dsrg_attention_paged_workspace: bad arguments");
+  if (B == 0 || Nq == 0) return 0;
+  const long long NC = (long long)Nq * (nh / p.H);
+  DSRG_CHECK(NC <= (1 << 20), "dsrg_attention_paged_workspace: %lld query rows per key / value head", NC);
+  const int ct = col_tiles((int)NC), cgs = (int)((NC + 16 * ct - 1) / (16 * ct));
+  const Split s = plan_split(B, p.H, cgs, seen_tokens(width, p.S, Nq, window));
+  return s.nsplit > 1 ? (int64_t)B * p.H * NC * s.nsplit * (cache->head_dim * 4 + 8) : 0;
+}
+
+extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q, int64_t q_bs, int q_rs, void* o, int64_t o_bs, int o_rs, float* lse,
+                                    const int32_t* table, int table_ld, int width, const int32_t* lens, int B, int nh, int Nq, float scale,
+                                    int causal, int window, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  PagedArgs a;
+  int rc = check_cache(cache, "dsrg_attention_paged", a.c);
+  if (rc) return rc;
+  DSRG_CHECK(dtype == (cache->dtype == DSRG_F32 ? DSRG_F32 : DSRG_BF16), "dsrg_attention_paged: queries of dtype %d for a cache of dtype %d", dtype, cache->dtype);
+  DSRG_CHECK(nh >= 1 && nh % a.c.H == 0, "dsrg_attention_paged: %d query heads over %d key / value heads", nh, a.c.H);
+  DSRG_CHECK(window >= 0 && (causal || !window), "dsrg_attention_paged: a window needs causal = 1 (window %d)", window);
+  if (B == 0 || Nq == 0) return DSRG_OK;
+  DSRG_CHECK(q && o && lens && B > 0 && B <= 65535 && Nq > 0, "dsrg_attention_paged: bad arguments");
+  if ((rc = check_table("dsrg_attention_paged", table, table_ld, width, a.c.S, B))) return rc;
+  const int size = dtype == DSRG_F32 ? 4 : 2, D_ = cache->head_dim;
+  DSRG_CHECK(rows16(q, q_bs, q_rs, size) && rows16(o, o_bs, o_rs, size), "dsrg_attention_paged: rows must be 16-byte aligned");
+  const int64_t need = dsrg_attention_paged_workspace(cache, width, B, nh, Nq, window);
+  if (need < 0) return (int)need;
+  DSRG_CHECK(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), "dsrg_attention_paged: workspace of %lld bytes needed, %lld given",
+             (long long)need, (long long)workspace_bytes);
+  a.G = nh / a.c.H;
+  a.NC = Nq * a.G;
+  const int ct = col_tiles(a.NC), cgs = (a.NC + 16 * ct - 1) / (16 * ct);
+  DSRG_CHECK((long long)a.c.H * cgs <= 65535, "dsrg_attention_paged: %d query rows per key / value head", a.NC);
+  const Split s = plan_split(B, a.c.H, cgs, seen_tokens(width, a.c.S, Nq, window));
+  a.q = q; a.o = o; a.lse = lse; a.q_bs = q_bs; a.o_bs = o_bs; a.q_rs = q_rs; a.o_rs = o_rs;
+  a.table = table; a.lens = lens; a.table_ld = table_ld; a.width = width; a.B = B; a.nh = nh; a.Nq = Nq;
+  a.causal = causal != 0; a.window = window; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
+  a.ws_o = (float*)workspace;
+  a.ws_ml = need ? (float2*)((float*)workspace + (int64_t)B * a.c.H * a.NC * s.nsplit * D_) : nullptr;
+  const dim3 grid(s.nsplit, a.c.H * cgs, B), block(256);
+  const hipStream_t st = (hipStream_t)stream;
+  const bool mix = causal && Nq > 1;
+  KV_SWITCH(cache->dtype, D_SWITCH(D_, {
+    if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true>), grid, block, 0, st, a);
+    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true>), grid, block, 0, st, a);
+    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false>), grid, block, 0, st, a);
+  }))
+  DSRG_LAUNCH_CHECK("dsrg_attention_paged");
+  if (s.nsplit > 1) {
+    const long long rows = (long long)B * a.c.H * a.NC;
+    const dim3 jgrid((unsigned)((rows + 3) / 4));
+    D_SWITCH(D_, {
+      if (dtype == DSRG_F32) hipLaunchKernelGGL((attention_paged_join_kernel<D, float>), jgrid, block, 0, st, a);
+      else hipLaunchKernelGGL((attention_paged_join_kernel<D, bf16_t>), jgrid, block, 0, st, a);
+    })
+    DSRG_LAUNCH_CHECK("dsrg_attention_paged (join)");
+  }
+  return DSRG_OK;
+}

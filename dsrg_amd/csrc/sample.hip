@@ -1,0 +1,317 @@
+// Draw of one entry per row of logits with temperature, top-k, top-p and min-p, from given random numbers (gfx950).
+//
+// The entries of a row in falling order (equal ones: the lowest index first) are cut three times, and each cut leaves a prefix of
+// that order: after the k-th entry; after the first whose running weight reaches p of what the first cut left; where the weight
+// falls under m times the largest.  So nothing is sorted: a cut is a threshold on the 64-bit number (value's order-preserving
+// bits, ~index), found from a histogram (count or weight per bin of max - x) and the exact ranks inside the one bin that the cut
+// falls into.  The draw is the inverse distribution function over what is left, in index order.
+// Weights exp((x - max) / T) are fixed-point numbers of 44 bits behind the point, from a double exponential: integer sums do not
+// depend on the order of the atomics, and 2^-45 an entry is far below what a 24-bit random number resolves.
+#include "common.h"
+#include <math.h>
+
+typedef unsigned long long u64;
+
+namespace {
+
+constexpr int LIST = 1024;           // entries of the cut's bin that are ranked directly
+constexpr int WBITS = 44;
+
+struct SampleArgs {
+  const void* logits;
+  long long ld;
+  const float* u;
+  const float* temp; const int32_t* topk; const float* topp; const float* minp;      // NULL: the number beside it
+  float temp0; int topk0; float topp0, minp0;
+  int64_t* token; float* logp;
+  int V;
+};
+
+__device__ __forceinline__ unsigned key_of(float x) {
+  const unsigned b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ u64 comp_of(float x, int j) { return ((u64)key_of(x) << 32) | (unsigned)~j; }
+
+// 2^t in WBITS-bit fixed point for t <= 0: 2^(n/32) from a table, 2^(r/32) = e^y with |y| <= ln2/64 by its series (the first
+// term left out is y^6 / 720 < 3e-15)
+__device__ __forceinline__ u64 fixed_exp2(double t, const double* tab) {
+  if (!(t > -46.0)) return 0;
+  const double s = rint(t * 32.0), y = (t - s * (1.0 / 32.0)) * 0.69314718055994530942;
+  const int n = (int)s;
+  double e = fma(y, 1.0 / 120.0, 1.0 / 24.0);
+  e = fma(y, e, 1.0 / 6.0);
+  e = fma(y, e, 0.5);
+  e = fma(y, e, 1.0);
+  e = fma(y, e, 1.0);
+  return (u64)__double2ll_rn(ldexp(e * tab[n & 31], (n >> 5) + WBITS));
+}
+
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ float load_logit(const T* row, int j) {
+  const float x = Elem<T>::ld(row + j) + 0.0f;          // (-0 + 0 = +0: the two zeros are one value)
+  return x != x ? -INFINITY : x;
+}
+
+template <typename T, int NT, int NB>
+__global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
+  constexpr int NW = NT / 64, BPT = NB / NT;            // bins per thread
+  __shared__ u64 mass[NB];
+  __shared__ unsigned cnt[NB];
+  __shared__ u64 l_comp[LIST], l_w[LIST];
+  __shared__ double tab[32];
+  __shared__ u64 red_a[NW], red_b[NW];
+  __shared__ u64 s_thr, s_base_m, s_base_c, s_bin_m;
+  __shared__ unsigned s_bin, s_n, s_bin_n;
+  __shared__ int s_pick;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
+  const T* row = (const T*)a.logits + (long long)b * a.ld;
+  const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
+  const int Kk = a.topk ? a.topk[b] : a.topk0;
+  if (tid < 32) tab[tid] = exp2(tid / 32.0);
+  // wave w's part of the row: index order is (wave, step, lane)
+  const int seg = (V + NW * 64 - 1) / (NW * 64) * 64, j0 = min(V, w * seg), j1 = min(V, j0 + seg);
+
+  // largest value, lowest index first, and how many entries can be drawn at all
+  u64 best = 0;
+  unsigned valid = 0;
+  for (int j = j0 + lane; j < j1; j += 64) {
+    const float x = load_logit(row, j);
+    if (x > -INFINITY) { ++valid; const u64 c = comp_of(x, j); best = c > best ? c : best; }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    const u64 c = __shfl_xor(best, o);
+    best = c > best ? c : best;
+    valid += __shfl_xor(valid, o);
+  }
+  if (lane == 0) { red_a[w] = best; red_b[w] = valid; }
+  __syncthreads();
+  best = 0;
+  u64 nvalid = 0;
+  for (int i = 0; i < NW; ++i) { best = red_a[i] > best ? red_a[i] : best; nvalid += red_b[i]; }
+  if (nvalid == 0) {                                    // nothing to draw from
+    if (tid == 0) { a.token[b] = -1; a.logp[b] = -INFINITY; }
+    return;
+  }
+  const float mx = of_key((unsigned)(best >> 32));
+  if (!(Tm > 0.f)) {                                    // greedy
+    if (tid == 0) { a.token[b] = (int)~(unsigned)best; a.logp[b] = 0.f; }
+    return;
+  }
+  const double c2 = 1.44269504088896340736 / (double)Tm;
+  auto weight = [&](float x) -> u64 { return x == mx ? (u64)1 << WBITS : fixed_exp2(((double)x - (double)mx) * c2, tab); };
+  // bins of max - x: its float bits from 2^-8 to 2^8, NB / 16 an octave (monotone in x, whatever the logits' spread)
+  constexpr int SH = 23 - (NB == 4096 ? 8 : NB == 1024 ? 6 : 0);
+  auto bin_of = [&](float x) -> unsigned {
+    const unsigned d = x == mx ? 0u : __float_as_uint(mx - x) >> SH;
+    const unsigned lo = 0x3b800000u >> SH;              // 2^-8
+    return d < lo ? 0u : min(d - lo, (unsigned)NB - 1);
+  };
+
+  // Running count and weight over the bins, behind (c0, m0); the first bin that reaches the goal goes to s_bin, with what lies
+  // before it and what it holds.  *goal < 0: it is frac of what all bins weigh.  (Entries so far down that their weight rounds to
+  // 0 never reach a goal: the last bin that weighs anything does.)
+  auto locate = [&](bool by_mass, u64 want, double frac, u64 c0, u64 m0, double* goal) {
+    u64 tc = 0, tm = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) { tc += cnt[tid * BPT + i]; tm += mass[tid * BPT + i]; }
+    u64 ic = tc, im = tm;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 yc = __shfl_up(ic, o), ym = __shfl_up(im, o);
+      if (lane >= o) { ic += yc; im += ym; }
+    }
+    if (lane == 63) { red_a[w] = ic; red_b[w] = im; }
+    __syncthreads();
+    u64 bc = c0, bm = m0, total = 0;
+    for (int i = 0; i < NW; ++i) { if (i < w) { bc += red_a[i]; bm += red_b[i]; } total += red_b[i]; }
+    ic += bc; im += bm;
+    u64 ec = ic - tc, em = im - tm;
+    if (*goal < 0) *goal = fmax(frac, 0.0) * (double)total;
+    if (tc && (by_mass ? ((double)em < *goal || ec == 0) && (double)im >= *goal : ec < want && ic >= want)) {
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        const u64 nc = cnt[tid * BPT + i], nm = mass[tid * BPT + i];
+        if (!done && nc && (by_mass ? (double)(em + nm) >= *goal : ec + nc >= want)) {
+          done = true;
+          s_bin = tid * BPT + i; s_base_c = ec; s_base_m = em; s_bin_n = (unsigned)nc; s_bin_m = nm;
+        }
+        ec += nc; em += nm;
+      }
+    }
+    __syncthreads();
+  };
+  u64 thr = 0;                                          // entries with comp >= thr are kept (comp of a valid entry is never 0)
+  // One cut: by_mass false: after `want` entries; true: after the first whose running weight reaches frac of the whole.
+  auto cut = [&](bool by_mass, u64 want, double frac) {
+    double goal = -1.0;
+    for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
+    if (tid == 0) { s_thr = ~0ull; s_n = 0; }
+    __syncthreads();
+    for (int j = j0 + lane; j < j1; j += 64) {
+      const float x = load_logit(row, j);
+      if (x > -INFINITY && comp_of(x, j) >= thr) {
+        const unsigned bin = bin_of(x);
+        atomicAdd(&cnt[bin], 1u);
+        if (by_mass) atomicAdd(&mass[bin], weight(x));
+      }
+    }
+    __syncthreads();
+    locate(by_mass, want, frac, 0, 0, &goal);
+    const unsigned bin = s_bin;
+    u64 base_c = s_base_c, base_m = s_base_m;
+    if (s_bin_n <= LIST) {
+      for (int j = j0 + lane; j < j1; j += 64) {
+        const float x = load_logit(row, j);
+        if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin) {
+          const unsigned at = atomicAdd(&s_n, 1u);
+          l_comp[at] = comp_of(x, j);
+          l_w[at] = by_mass ? weight(x) : 0;
+        }
+      }
+      __syncthreads();
+      const int n = (int)s_n;
+      for (int i = tid; i < n; i += NT) {
+        const u64 me = l_comp[i];
+        u64 c = base_c, m = base_m;
+        for (int k = 0; k < n; ++k)
+          if (l_comp[k] > me) { ++c; m += l_w[k]; }
+        if (by_mass ? (double)m < goal || c == 0 : c < want) atomicMin(&s_thr, me);
+      }
+      __syncthreads();
+      thr = s_thr;
+    } else {
+      // many entries in one bin (a flat row, or equal values): by the value's 32 bits, LB of them a pass
+      constexpr int LB = NB == 4096 ? 12 : 10;
+      unsigned prefix = 0, pmask = 0;
+      for (int sh = 32; sh > 0;) {
+        const int nb = min(LB, sh);
+        sh -= nb;
+        for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
+        __syncthreads();
+        for (int j = j0 + lane; j < j1; j += 64) {
+          const float x = load_logit(row, j);
+          const unsigned k = key_of(x);
+          if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin && (k & pmask) == prefix) {
+            const unsigned dig = ~(k >> sh) & ((1u << nb) - 1);            // falling values
+            atomicAdd(&cnt[dig], 1u);
+            if (by_mass) atomicAdd(&mass[dig], weight(x));
+          }
+        }
+        __syncthreads();
+        locate(by_mass, want, frac, base_c, base_m, &goal);
+        base_c = s_base_c; base_m = s_base_m;
+        prefix |= (~s_bin & ((1u << nb) - 1)) << sh;
+        pmask |= ((1u << nb) - 1) << sh;
+        __syncthreads();
+      }
+      // s_bin_n equal values of weight s_bin_m / s_bin_n: as many of them as the goal asks, the lowest indices first
+      u64 r;
+      const u64 each = s_bin_m / s_bin_n;
+      if (by_mass) {
+        const double left = goal - (double)base_m;
+        r = each && left > 0 ? (u64)ceil(left / (double)each) : 1;
+        while (r > 1 && (double)(base_m + (r - 1) * each) >= goal) --r;
+        while ((double)(base_m + r * each) < goal && r < s_bin_n) ++r;
+      } else r = want - base_c;
+      if (r < 1) r = 1;
+      if (r > s_bin_n) r = s_bin_n;
+      unsigned mine = 0;
+      for (int j = j0 + lane; j - lane < j1; j += 64) mine += __popcll(__ballot(j < j1 && key_of(load_logit(row, j < V ? j : V - 1)) == prefix));
+      if (lane == 0) red_a[w] = mine;
+      __syncthreads();
+      u64 before = 0;
+      for (int i = 0; i < w; ++i) before += red_a[i];
+      if (before < r && before + mine >= r) {           // this wave holds the r-th of them
+        u64 left = r - before;
+        for (int j = j0 + lane; j - lane < j1; j += 64) {
+          const u64 hit = __ballot(j < j1 && key_of(load_logit(row, j < V ? j : V - 1)) == prefix);
+          const u64 n = __popcll(hit);
+          if (left <= n) {
+            if ((hit >> lane & 1) && __popcll(hit & (((u64)1 << lane) - 1)) == left - 1) s_thr = ((u64)prefix << 32) | (unsigned)~j;
+            break;
+          }
+          left -= n;
+        }
+      }
+      __syncthreads();
+      thr = s_thr;
+    }
+    __syncthreads();
+  };
+  if (Kk > 0 && (u64)Kk < nvalid) cut(false, (u64)Kk, 0.0);
+  if (P < 1.f) cut(true, 0, (double)P);
+  const double floor_ = M > 0.f ? (double)mx + (double)Tm * log((double)M) : -INFINITY;        // w >= m  <=>  x >= max + T ln m
+
+  // what is left, in index order
+  u64 sum = 0;
+  auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
+  __syncthreads();
+  for (int j = j0 + lane; j < j1; j += 64) {
+    const float x = load_logit(row, j);
+    if (kept(x, j)) sum += weight(x);
+  }
+  sum = wave_sum_u64(sum);
+  if (lane == 0) red_a[w] = sum;
+  __syncthreads();
+  u64 total = 0, before = 0;
+  for (int i = 0; i < NW; ++i) { if (i < w) before += red_a[i]; total += red_a[i]; }
+  float uu = a.u[b];
+  uu = uu >= 0.f ? fminf(uu, 0.99999994f) : 0.f;
+  const double goal = (double)uu * (double)total;
+  if (sum && (double)before <= goal && (double)(before + sum) > goal) {       // one wave: the running sums rise
+    u64 base = before;
+    for (int s0 = j0; s0 < j1; s0 += 64) {
+      const int j = s0 + lane;
+      const float x = j < j1 ? load_logit(row, j) : -INFINITY;
+      const bool in = j < j1 && kept(x, j);
+      if (!__ballot(in)) continue;
+      u64 c = in ? weight(x) : 0;
+      const u64 own = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(c, o); if (lane >= o) c += y; }
+      const u64 hit = __ballot(own && (double)(base + c) > goal);
+      if (hit) {
+        if (lane == __builtin_ctzll(hit)) {
+          a.token[b] = j;
+          a.logp[b] = (float)((x == mx ? 0.0 : ((double)x - (double)mx) / (double)Tm) - log(ldexp((double)total, -WBITS)));
+        }
+        break;
+      }
+      base += __shfl(c, 63);
+    }
+  }
+}
+
+template <typename T> void launch(const SampleArgs& a, int B, hipStream_t st) {
+  if (a.V <= 4096) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024>), dim3(B), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096>), dim3(B), dim3(1024), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature, float temperature0,
+                                const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
+                                int64_t* token, float* logp, int B, int V, void* stream) {
+  DSRG_CHECK(dtype == DSRG_F32 || dtype == DSRG_BF16, "dsrg_sample_rows: unsupported dtype %d", dtype);
+  DSRG_CHECK(B >= 0 && V >= 1 && V <= (1 << 19), "dsrg_sample_rows: %d x %d logits (1 to 524288 a row)", B, V);
+  if (B == 0) return DSRG_OK;
+  DSRG_CHECK(logits && u && token && logp && (ld >= V || B == 1), "dsrg_sample_rows: bad arguments");
+  DSRG_CHECK(temperature || (temperature0 >= 0.f && temperature0 < INFINITY), "dsrg_sample_rows: temperature %g", (double)temperature0);
+  DSRG_CHECK(top_k || top_k0 >= 0, "dsrg_sample_rows: top_k %d", top_k0);
+  DSRG_CHECK(top_p || top_p0 >= 0.f, "dsrg_sample_rows: top_p %g", (double)top_p0);
+  DSRG_CHECK(min_p || (min_p0 >= 0.f && min_p0 <= 1.f), "dsrg_sample_rows: min_p %g", (double)min_p0);
+  const SampleArgs a{logits, ld, u, temperature, top_k, top_p, min_p, temperature0, top_k0, top_p0, min_p0, token, logp, V};
+  if (dtype == DSRG_F32) launch<float>(a, B, (hipStream_t)stream);
+  else launch<bf16_t>(a, B, (hipStream_t)stream);
+  DSRG_LAUNCH_CHECK("dsrg_sample_rows");
+  return DSRG_OK;
+}

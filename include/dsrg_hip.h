@@ -20,9 +20,10 @@
 extern "C" {
 #endif
 
-#define DSRG_ABI_VERSION 14
+#define DSRG_ABI_VERSION 15
 
-enum { DSRG_F32 = 0, DSRG_BF16 = 1 };
+enum { DSRG_F32 = 0, DSRG_BF16 = 1,
+       DSRG_I8 = 2, DSRG_E4M3 = 3 /* OCP 8-bit float; these two only as the storage of a key / value cache */ };
 enum { DSRG_OK = 0, DSRG_EINVAL = -1, DSRG_ELAUNCH = -2, DSRG_EUNSUPPORTED = -3 };
 
 int dsrg_abi_version(void);
@@ -356,6 +357,57 @@ int dsrg_nav_logits_fwd_og(const float* g_raw, const float* l_raw, const float* 
 int dsrg_action_tail_fwd(const float* logits, int ld, const int64_t* targets, int64_t ignore_index, const float* u,
                          float* stop_prob, int32_t* argmax, int32_t* sample, float* entropy, float* loss_rows,
                          float* dlogits, int B, int N, void* stream);
+
+/* ---- draw of one entry per row with temperature, top-k, top-p and min-p -------------------------------------------
+ * The filtered form of the draw above (the rollout's 'sample' feedback, FT/r2r/agent.py:511-514), and of a word of the vocabulary.
+ * logits [B,V] (row stride ld, dtype DSRG_F32 / DSRG_BF16; -inf and NaN = not a candidate), u fp32 [B] in [0, 1).  temperature,
+ * top_k, top_p and min_p: fp32 / int32 device arrays [B], or NULL for the number beside them.  The candidates in falling order
+ * (equal values: the lowest index first) are cut (1) after the k-th (k <= 0: no cut); (2) after the first whose running sum of
+ * weights w = exp((x - max) / T) reaches p of the sum over what (1) left (p >= 1: no cut; the first one always stays); (3) before
+ * the first with w < m (m <= 0: no cut).  token[b] = the first entry, in index order, at which the running sum over what is left
+ * exceeds u[b] times the whole; logp[b] = its log-probability among them.  T <= 0 (or NaN): the largest entry, logp 0.  A row without
+ * a candidate: token -1, logp -inf.  1 <= V <= 524288.  Deterministic: sums are 64-bit integers. */
+int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature, float temperature0,
+                     const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
+                     int64_t* token, float* logp, int B, int V, void* stream);
+
+/* ---- paged key / value cache (no counterpart in the reference, which keeps padded dense tensors) --------------------
+ * Pages of `page_size` tokens (a power of two, 32 or more) hold the keys and values of all heads; token t of sequence b lies in
+ * page table[b * table_ld + t / page_size], row t % page_size; a table has `width` entries a sequence.  Inside (page, head):
+ *   bf16 and 8 bits:  K [S/16][D/8][16 tokens][8 dims]; V [S/32][D/16][4 g][16 dims][2 m][4 i], token 32 t + 16 m + 4 g + i;
+ *   fp32:             K [S/16][D/4][16 tokens][4 dims]; V [S/16][D/16][4 g][16 dims][4 i],      token 16 t + 4 g + i;
+ * k_scale / v_scale fp32 [n_pages][n_kv_heads][page_size] (8-bit dtypes only, else NULL): value = code * scale, with
+ * scale = max(largest magnitude of the token's head row * (1/127 | 1/448), 2^-126); a row that holds a NaN or an infinity gets the
+ * scale NaN and reads as NaN.  head_dim 64 or 128.  Buffers are 16-byte aligned.  Whatever lies on pages that no table names, or past a
+ * sequence's length, is never used; a table entry outside [0, n_pages) is a page that is not there: nothing is written to
+ * it, it reads as zero, attention does not see its tokens. */
+typedef struct {
+  void* k_pool; void* v_pool;
+  float* k_scale; float* v_scale;
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+  int32_t dtype;          /* DSRG_F32, DSRG_BF16, DSRG_I8, DSRG_E4M3 */
+  int32_t reserved_;
+} dsrg_kv_cache_t;
+/* Writes row t < count[b] (count NULL: T) of k / v [B, T, n_kv_heads * head_dim] (batch / row strides free, 16-byte aligned rows, the
+ * heads of a row side by side) as token start[b] + t of sequence b.  dtype of the rows: the cache's, or either one for 8 bits.  Rows past
+ * the table's end are dropped.  Two rows of one call must not name the same token of the same page. */
+int dsrg_kv_append(const dsrg_kv_cache_t* cache, const void* k, int64_t k_bs, int k_rs, const void* v, int64_t v_bs, int v_rs, int dtype,
+                   const int32_t* table, int table_ld, int width, const int32_t* start, const int32_t* count, int B, int T, void* stream);
+/* The tokens start[b] + t (start NULL: t), t < count[b], as dense rows k / v [B, N, n_kv_heads * head_dim]; rows t >= count[b] are zero. */
+int dsrg_kv_read(const dsrg_kv_cache_t* cache, void* k, int64_t k_bs, int k_rs, void* v, int64_t v_bs, int v_rs, int dtype,
+                 const int32_t* table, int table_ld, int width, const int32_t* start, const int32_t* count, int B, int N, void* stream);
+/* o[b,i,h] = softmax over the tokens t that row i sees of (scale * q[b,i,h] . k[t, h / G]), times v[t, h / G]; G = nh / n_kv_heads.
+ * q, o [B, Nq, nh * head_dim] in dtype (fp32 for an fp32 cache, else bf16).  A row sees the tokens t < lens[b]; with causal = 1 row i
+ * stands at position p = lens[b] - Nq + i (the Nq rows are the newest tokens, already in the cache) and sees t <= p, with window > 0
+ * only t > p - window.  lens is clamped to the table's reach.  Rows that see nothing: o = 0, lse = -inf.  lse fp32 [B,nh,Nq] or
+ * NULL: log-sum-exp of the scaled scores.  Scores, sums and O are held in fp32; bf16 / 8-bit caches round P (times the value's
+ * scale) to bf16 for the matrix instruction.  Few rows: the tokens are split over workgroups and joined by a second kernel, through a
+ * workspace of dsrg_attention_paged_workspace() bytes (0: none needed; negative: an error code) that belongs to this call until
+ * it has run: two calls that may overlap need two. */
+int64_t dsrg_attention_paged_workspace(const dsrg_kv_cache_t* cache, int width, int B, int nh, int Nq, int window);
+int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q, int64_t q_bs, int q_rs, void* o, int64_t o_bs, int o_rs, float* lse,
+                         const int32_t* table, int table_ld, int width, const int32_t* lens, int B, int nh, int Nq, float scale,
+                         int causal, int window, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /* Cross-entropy rows = F.cross_entropy(logits, targets, ignore_index, reduction='none') of the pre-training losses
  * (PT/model/pretrain_cmt.py:160-167 MLM over the vocabulary, :286-294 the three SAP terms, :325 OG).  logits fp32 [B,N]
