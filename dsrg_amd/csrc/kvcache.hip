@@ -74,6 +74,24 @@ template <int D> __device__ __forceinline__ float row_max(float v) {
   return v;
 }
 
+// What is stored of 8 dims of a row (its D / 8 lanes call this together), and the row's scale
+template <int KV, int D, typename TS> __device__ __forceinline__ void encode(const float (&x)[8], TS (&w)[8], int d0, float* scale, long long at) {
+  if constexpr (KvT<KV>::SZ == 1) {
+    float m = 0.f;
+    bool fin = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { m = fmaxf(m, fabsf(x[j])); fin = fin && fabsf(x[j]) <= 3.4028235e38f; }
+    m = row_max<D>(fin ? m : INFINITY);
+    const float s = kv_scale<KV>(m, m <= 3.4028235e38f);
+    if (d0 == 0) scale[at] = s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = (TS)kv_code<KV>(x[j], s);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) Elem<TS>::st(&w[j], x[j]);
+  }
+}
+
 // ---- write ---------------------------------------------------------------------------------------------------------------
 struct AppendArgs {
   Pool c;
@@ -108,20 +126,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     ld8(src, x);
     TS* dst = (TS*)(which ? a.c.v : a.c.k) + ph * a.c.S * D;
     TS w[8];
-    if (KvT<KV>::SZ == 1) {
-      float m = 0.f;
-      bool fin = true;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) { m = fmaxf(m, fabsf(x[j])); fin = fin && fabsf(x[j]) <= 3.4028235e38f; }
-      m = row_max<D>(fin ? m : INFINITY);
-      const float s = kv_scale<KV>(m, m <= 3.4028235e38f);
-      if (d0 == 0) (which ? a.c.vs : a.c.ks)[ph * a.c.S + r] = s;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = (TS)kv_code<KV>(x[j], s);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) Elem<typename std::conditional<KV == DSRG_F32, float, bf16_t>::type>::st((typename std::conditional<KV == DSRG_F32, float, bf16_t>::type*)&w[j], x[j]);
-    }
+    encode<KV, D>(x, w, d0, which ? a.c.vs : a.c.ks, ph * a.c.S + r);
     if (which == 0) {
 #pragma unroll
       for (int j = 0; j < 8; j += KvT<KV>::E) __builtin_memcpy(__builtin_assume_aligned(dst + k_off<KV, D>(r, d0 + j), KvT<KV>::E * KvT<KV>::SZ), &w[j], KvT<KV>::E * KvT<KV>::SZ);
@@ -129,6 +134,70 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) dst[v_off<KV, D>(r, d0 + j)] = w[j];
     }
+  }
+}
+
+// A 32-token block of values on its way between rows and the pool's order: runs of 16 dims (one lane group of one dim tile) lie 16
+// (8-bit: 8) bytes further apart than in the pool, so that the lanes of a row write to different LDS banks.
+template <int KV, int D> struct VTile {
+  static constexpr int E = KvT<KV>::E, RUN = 16 * E, STRIDE = RUN + (KvT<KV>::SZ == 4 ? 4 : 8), SIZE = 32 * D / RUN * STRIDE;
+  __device__ static __forceinline__ int at(int off) { return off / RUN * STRIDE + off % RUN; }
+};
+
+// Many tokens of a sequence: one workgroup per (sequence, aligned 32-token block, head).  The block's rows are read whole, go through LDS
+// into the pool's order and leave as whole chunks; a chunk of 8 (4) tokens that the call covers in part is written element by
+// element, so that its other tokens stay.
+template <int KV, int D, typename TI>
+__global__ __launch_bounds__(256) void kv_append_block_kernel(const AppendArgs a) {
+  typedef typename KvT<KV>::type TS;
+  typedef VTile<KV, D> VT;
+  constexpr int LPR = D / 8, RPP = 256 / LPR, E = KvT<KV>::E, SZ = KvT<KV>::SZ;
+  __shared__ __attribute__((aligned(16))) TS sk[32 * D];
+  __shared__ __attribute__((aligned(16))) TS sv[VT::SIZE];
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const long long start = a.start[b], lo = max(start, 0ll);
+  const long long hi = min(start + (a.count ? min(a.count[b], a.T) : a.T), (long long)a.width * a.c.S);
+  const long long pos0 = (lo & ~31ll) + 32ll * blockIdx.x;
+  if (pos0 >= hi) return;
+  const int page = a.table[(long long)b * a.table_ld + (pos0 >> a.c.lgS)];
+  if (page < 0 || page >= a.c.P) return;
+  const long long ph = (long long)page * a.c.H + h;
+  const int in_page = (int)pos0 & (a.c.S - 1);
+  const int v0 = (int)max(lo - pos0, 0ll), v1 = (int)min(hi - pos0, 32ll);          // the block's rows that the call writes
+  const int d0 = (tid % LPR) * 8;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += RPP) {
+      const int r = r0 + tid / LPR;
+      if (r < v0 || r >= v1) continue;
+      const TI* src = (const TI*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (pos0 + r - start) * (which ? a.v_rs : a.k_rs) + h * D + d0;
+      float x[8];
+      ld8(src, x);
+      TS w[8];
+      encode<KV, D>(x, w, d0, (which ? a.c.vs : a.c.ks), ph * a.c.S + in_page + r);
+      if (which == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; j += E) __builtin_memcpy(__builtin_assume_aligned(sk + k_off<KV, D>(r, d0 + j), E * SZ), &w[j], E * SZ);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sv[VT::at(v_off<KV, D>(r, d0 + j))] = w[j];
+      }
+    }
+  __syncthreads();
+  const unsigned vm = (v1 >= 32 ? ~0u : (1u << v1) - 1) & ~((1u << v0) - 1);
+  TS* kd = (TS*)a.c.k + (ph * a.c.S + in_page) * D;
+  TS* vd = (TS*)a.c.v + (ph * a.c.S + in_page) * D;
+  for (int q = tid; q < 32 * D / E; q += 256) {
+    const int r = q / (D / E * 16) * 16 + q % 16;
+    if (vm >> r & 1) __builtin_memcpy(__builtin_assume_aligned(kd + q * E, E * SZ), __builtin_assume_aligned(sk + q * E, E * SZ), E * SZ);
+    const int g = q / 16 % 4;
+    const unsigned m = E == 8 ? (vm >> 4 * g & 15) | (vm >> (16 + 4 * g) & 15) << 4 : vm >> (q / (D * 4) * 16 + 4 * g) & 15;
+    const TS* from = sv + VT::at(q * E);
+    if (m == (1u << E) - 1) __builtin_memcpy(__builtin_assume_aligned(vd + q * E, E * SZ), __builtin_assume_aligned(from, E * SZ), E * SZ);
+    else if (m)
+      for (int j = 0; j < E; ++j)
+        if (m >> j & 1) vd[q * E + j] = from[j];
   }
 }
 
@@ -142,42 +211,63 @@ struct ReadArgs {
   int table_ld, width, B, N;
 };
 
-// Same lanes as the write; a row past the sequence's count (or on no page) is zero.
+// One workgroup per (sequence, aligned 32-token block, head): values come as whole chunks and are turned into rows through LDS, a
+// key chunk is a piece of a row already.  A row past the sequence's count (or on no page) is zero.
 template <int KV, int D, typename TO>
 __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
   typedef typename KvT<KV>::type TS;
-  constexpr int LPR = D / 8;
-  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int d0 = (threadIdx.x % LPR) * 8, H = a.c.H;
-  if (row >= (long long)a.B * a.N * H) return;
-  const int h = (int)(row % H);
-  const long long bt = row / H;
-  const int b = (int)(bt / a.N), t = (int)(bt % a.N);
-  const long long pos = (long long)(a.start ? a.start[b] : 0) + t;
+  typedef VTile<KV, D> VT;
+  constexpr int LPR = D / 8, RPP = 256 / LPR, E = KvT<KV>::E, SZ = KvT<KV>::SZ;
+  __shared__ __attribute__((aligned(16))) TS sv[VT::SIZE];
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const long long start = a.start ? a.start[b] : 0, pos0 = (start & ~31ll) + 32ll * blockIdx.x;
+  if (pos0 - start >= a.N) return;
+  const int count = min(a.count[b], a.N);
   int page = -1;
-  if (t < a.count[b] && pos >= 0 && pos < (long long)a.width * a.c.S) page = a.table[(long long)b * a.table_ld + (pos >> a.c.lgS)];
-  const bool live = page >= 0 && page < a.c.P;
-  const int r = (int)pos & (a.c.S - 1);
-  const long long ph = (long long)page * H + h;
+  if (pos0 >= 0 && pos0 < (long long)a.width * a.c.S && pos0 - start < count) page = a.table[(long long)b * a.table_ld + (pos0 >> a.c.lgS)];
+  const bool there = page >= 0 && page < a.c.P;
+  const long long ph = (long long)page * a.c.H + h, row0 = ph * a.c.S + ((int)pos0 & (a.c.S - 1));
+  if (there) {
+    const TS* vs = (const TS*)a.c.v + row0 * D;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (live) {
-      const TS* src = (const TS*)(which ? a.c.v : a.c.k) + ph * a.c.S * D;
-      const float s = KvT<KV>::SZ == 1 ? (which ? a.c.vs : a.c.ks)[ph * a.c.S + r] : 1.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const TS e = src[which ? v_off<KV, D>(r, d0 + j) : k_off<KV, D>(r, d0 + j)];
-        if constexpr (KvT<KV>::SZ == 1) x[j] = kv_value<KV>(e) * s;
-        else x[j] = Elem<TS>::ld(&e);
-      }
+    for (int q0 = 0; q0 < 32 * D / E; q0 += 256) {
+      const int q = q0 + tid;
+      __builtin_memcpy(__builtin_assume_aligned(sv + VT::at(q * E), E * SZ), __builtin_assume_aligned(vs + q * E, E * SZ), E * SZ);
     }
-    TO* dst = (TO*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (long long)t * (which ? a.v_rs : a.k_rs) + h * D + d0;
-    st4(dst, make_float4(x[0], x[1], x[2], x[3]));
-    st4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+    __syncthreads();
   }
+  const int d0 = (tid % LPR) * 8;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += RPP) {
+      const int r = r0 + tid / LPR;
+      const long long t = pos0 + r - start;
+      if (t < 0 || t >= a.N) continue;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (there && t < count) {
+        TS e[8];
+        if (which == 0) {
+          const TS* ks = (const TS*)a.c.k + row0 * D;
+#pragma unroll
+          for (int j = 0; j < 8; j += E) __builtin_memcpy(&e[j], __builtin_assume_aligned(ks + k_off<KV, D>(r, d0 + j), E * SZ), E * SZ);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = sv[VT::at(v_off<KV, D>(r, d0 + j))];
+        }
+        const float s = SZ == 1 ? (which ? a.c.vs : a.c.ks)[row0 + r] : 1.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (SZ == 1) x[j] = kv_value<KV>(e[j]) * s;
+          else x[j] = Elem<TS>::ld(&e[j]);
+        }
+      }
+      TO* dst = (TO*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + t * (which ? a.v_rs : a.k_rs) + h * D + d0;
+      st4(dst, make_float4(x[0], x[1], x[2], x[3]));
+      st4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+    }
 }
 
 // ---- attention over the cache ----------------------------------------------------------------------------------------------
@@ -606,14 +696,21 @@ extern "C" int dsrg_kv_append(const dsrg_kv_cache_t* cache, const void* k, int64
   DSRG_CHECK(rows16(k, k_bs, k_rs, size) && rows16(v, v_bs, v_rs, size), "dsrg_kv_append: rows must be 16-byte aligned");
   a.k = k; a.v = v; a.k_bs = k_bs; a.v_bs = v_bs; a.k_rs = k_rs; a.v_rs = v_rs;
   a.table = table; a.start = start; a.count = count; a.table_ld = table_ld; a.width = width; a.B = B; a.T = T;
-  const long long threads = (long long)B * T * a.c.H * (cache->head_dim / 8), blocks = (threads + 255) / 256;
-  DSRG_CHECK(blocks < (1ll << 31), "dsrg_kv_append: %lld rows in one call", (long long)B * T);
-  const dim3 grid((unsigned)blocks), block(256);
+  DSRG_CHECK(B <= 65535 && a.c.H <= 65535, "dsrg_kv_append: %d sequences of %d heads in one call", B, a.c.H);
+  const bool rows = T < 8;
+  const long long threads = (long long)B * T * a.c.H * (cache->head_dim / 8);
+  const dim3 grid = rows ? dim3((unsigned)((threads + 255) / 256)) : dim3((T + 31) / 32 + 1, a.c.H, B), block(256);
+  const hipStream_t st = (hipStream_t)stream;
   KV_SWITCH(cache->dtype, D_SWITCH(cache->head_dim, {
-    if constexpr (KV == DSRG_F32) hipLaunchKernelGGL((kv_append_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
-    else if constexpr (KV == DSRG_BF16) hipLaunchKernelGGL((kv_append_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
-    else if (dtype == DSRG_F32) hipLaunchKernelGGL((kv_append_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((kv_append_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);
+    auto go = [&](auto ti) {
+      typedef decltype(ti) TI;
+      if (rows) hipLaunchKernelGGL((kv_append_kernel<KV, D, TI>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((kv_append_block_kernel<KV, D, TI>), grid, block, 0, st, a);
+    };
+    if constexpr (KV == DSRG_F32) go(0.f);
+    else if constexpr (KV == DSRG_BF16) go((bf16_t)0);
+    else if (dtype == DSRG_F32) go(0.f);
+    else go((bf16_t)0);
   }))
   DSRG_LAUNCH_CHECK("dsrg_kv_append");
   return DSRG_OK;
@@ -632,9 +729,8 @@ extern "C" int dsrg_kv_read(const dsrg_kv_cache_t* cache, void* k, int64_t k_bs,
   DSRG_CHECK(rows16(k, k_bs, k_rs, size) && rows16(v, v_bs, v_rs, size), "dsrg_kv_read: rows must be 16-byte aligned");
   a.k = k; a.v = v; a.k_bs = k_bs; a.v_bs = v_bs; a.k_rs = k_rs; a.v_rs = v_rs;
   a.table = table; a.start = start; a.count = count; a.table_ld = table_ld; a.width = width; a.B = B; a.N = N;
-  const long long threads = (long long)B * N * a.c.H * (cache->head_dim / 8), blocks = (threads + 255) / 256;
-  DSRG_CHECK(blocks < (1ll << 31), "dsrg_kv_read: %lld rows in one call", (long long)B * N);
-  const dim3 grid((unsigned)blocks), block(256);
+  DSRG_CHECK(B <= 65535 && a.c.H <= 65535, "dsrg_kv_read: %d sequences of %d heads in one call", B, a.c.H);
+  const dim3 grid((N + 31) / 32 + 1, a.c.H, B), block(256);
   KV_SWITCH(cache->dtype, D_SWITCH(cache->head_dim, {
     if constexpr (KV == DSRG_F32) hipLaunchKernelGGL((kv_read_kernel<KV, D, float>), grid, block, 0, (hipStream_t)stream, a);
     else if constexpr (KV == DSRG_BF16) hipLaunchKernelGGL((kv_read_kernel<KV, D, bf16_t>), grid, block, 0, (hipStream_t)stream, a);

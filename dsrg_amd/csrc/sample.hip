@@ -34,18 +34,18 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ u64 comp_of(float x, int j) { return ((u64)key_of(x) << 32) | (unsigned)~j; }
 
-// 2^t in WBITS-bit fixed point for t <= 0: 2^(n/32) from a table, 2^(r/32) = e^y with |y| <= ln2/64 by its series (the first
-// term left out is y^6 / 720 < 3e-15)
-__device__ __forceinline__ u64 fixed_exp2(double t, const double* tab) {
-  if (!(t > -46.0)) return 0;
-  const double s = rint(t * 32.0), y = (t - s * (1.0 / 32.0)) * 0.69314718055994530942;
+// 2^(t32 / 32) in WBITS-bit fixed point for t32 <= 0: 2^(n/32) from a table, the rest as e^y, |y| <= ln2 / 64, by its series (the
+// first term left out is y^5 / 120 < 1.3e-12 of the weight).  Adding 2^(52 - WBITS) leaves the rounded fixed-point number in the mantissa.
+__device__ __forceinline__ u64 fixed_exp2(double t32, const double* tab) {
+  if (!(t32 > -46.0 * 32)) return 0;
+  const double s = rint(t32), y = (t32 - s) * (0.69314718055994530942 / 32);
   const int n = (int)s;
-  double e = fma(y, 1.0 / 120.0, 1.0 / 24.0);
-  e = fma(y, e, 1.0 / 6.0);
+  double e = fma(y, 1.0 / 24.0, 1.0 / 6.0);
   e = fma(y, e, 0.5);
   e = fma(y, e, 1.0);
   e = fma(y, e, 1.0);
-  return (u64)__double2ll_rn(ldexp(e * tab[n & 31], (n >> 5) + WBITS));
+  constexpr double MAGIC = (double)(1ull << (52 - WBITS));
+  return (u64)__double_as_longlong(ldexp(e * tab[n & 31], n >> 5) + MAGIC) - (u64)__builtin_bit_cast(long long, MAGIC);
 }
 
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
@@ -59,7 +59,9 @@ template <typename T> __device__ __forceinline__ float load_logit(const T* row, 
   return x != x ? -INFINITY : x;
 }
 
-template <typename T, int NT, int NB>
+// Where the row is: VPT > 0: a thread holds VPT values of it in registers for the passes of the short way (top-k with a small k, short
+// rows); the long way, taken by the others, reads the row again from the cache, eight independent loads at a time.
+template <typename T, int NT, int NB, int VPT>
 __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   constexpr int NW = NT / 64, BPT = NB / NT;            // bins per thread
   __shared__ u64 mass[NB];
@@ -69,22 +71,48 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   __shared__ u64 red_a[NW], red_b[NW];
   __shared__ u64 s_thr, s_base_m, s_base_c, s_bin_m;
   __shared__ unsigned s_bin, s_n, s_bin_n;
-  __shared__ int s_pick;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
   const T* row = (const T*)a.logits + (long long)b * a.ld;
   const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
   const int Kk = a.topk ? a.topk[b] : a.topk0;
+  const float u_raw = a.u[b], uu = u_raw >= 0.f ? fminf(u_raw, 0.99999994f) : 0.f;
   if (tid < 32) tab[tid] = exp2(tid / 32.0);
   // wave w's part of the row: index order is (wave, step, lane)
   const int seg = (V + NW * 64 - 1) / (NW * 64) * 64, j0 = min(V, w * seg), j1 = min(V, j0 + seg);
 
-  // largest value, lowest index first, and how many entries can be drawn at all
-  u64 best = 0;
-  unsigned valid = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const float x = load_logit(row, j);
-    if (x > -INFINITY) { ++valid; const u64 c = comp_of(x, j); best = c > best ? c : best; }
+  // f(value, index) for this thread's share of the row; -inf stands for what is no candidate
+  auto again = [&](auto&& f) {
+    for (int jb = j0 + lane; jb - lane < j1; jb += 512) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = load_logit(row, min(jb + i * 64, V - 1));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f(jb + i * 64 < j1 ? x[i] : -INFINITY, jb + i * 64);
+    }
+  };
+  float xs[VPT ? VPT : 1];
+  if constexpr (VPT > 0) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) xs[i] = load_logit(row, min(j0 + i * 64 + lane, V - 1));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) xs[i] = j0 + i * 64 + lane < j1 ? xs[i] : -INFINITY;
   }
+  auto each = [&](auto&& f) {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) f(xs[i], j0 + i * 64 + lane);
+    } else again(f);
+  };
+
+  // largest value, lowest index first, and how many entries can be drawn at all
+  float tmax = -INFINITY;
+  int tj = 0;
+  unsigned valid = 0;
+  each([&](float x, int j) {
+    valid += x > -INFINITY;
+    if (x > tmax) { tmax = x; tj = j; }                 // (a thread's indices rise)
+  });
+  u64 best = tmax > -INFINITY ? comp_of(tmax, tj) : 0;
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
     const u64 c = __shfl_xor(best, o);
@@ -95,6 +123,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   __syncthreads();
   best = 0;
   u64 nvalid = 0;
+#pragma unroll
   for (int i = 0; i < NW; ++i) { best = red_a[i] > best ? red_a[i] : best; nvalid += red_b[i]; }
   if (nvalid == 0) {                                    // nothing to draw from
     if (tid == 0) { a.token[b] = -1; a.logp[b] = -INFINITY; }
@@ -105,15 +134,20 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     if (tid == 0) { a.token[b] = (int)~(unsigned)best; a.logp[b] = 0.f; }
     return;
   }
-  const double c2 = 1.44269504088896340736 / (double)Tm;
+  const double c2 = 32 * 1.44269504088896340736 / (double)Tm;
   auto weight = [&](float x) -> u64 { return x == mx ? (u64)1 << WBITS : fixed_exp2(((double)x - (double)mx) * c2, tab); };
+  auto logp_of = [&](float x, u64 total) -> float {
+    return (float)((x == mx ? 0.0 : ((double)x - (double)mx) / (double)Tm) - log(ldexp((double)total, -WBITS)));
+  };
   // bins of max - x: its float bits from 2^-8 to 2^8, NB / 16 an octave (monotone in x, whatever the logits' spread)
-  constexpr int SH = 23 - (NB == 4096 ? 8 : NB == 1024 ? 6 : 0);
+  constexpr int SH = 23 - (NB == 4096 ? 8 : 6);
+  static_assert(NB == 4096 || NB == 1024, "NB / 16 bins an octave");
   auto bin_of = [&](float x) -> unsigned {
     const unsigned d = x == mx ? 0u : __float_as_uint(mx - x) >> SH;
     const unsigned lo = 0x3b800000u >> SH;              // 2^-8
     return d < lo ? 0u : min(d - lo, (unsigned)NB - 1);
   };
+  const double floor_ = M > 0.f ? (double)mx + (double)Tm * log((double)M) : -INFINITY;        // w >= m  <=>  x >= max + T ln m
 
   // Running count and weight over the bins, behind (c0, m0); the first bin that reaches the goal goes to s_bin, with what lies
   // before it and what it holds.  *goal < 0: it is frac of what all bins weigh.  (Entries so far down that their weight rounds to
@@ -156,27 +190,25 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
     if (tid == 0) { s_thr = ~0ull; s_n = 0; }
     __syncthreads();
-    for (int j = j0 + lane; j < j1; j += 64) {
-      const float x = load_logit(row, j);
+    again([&](float x, int j) {
       if (x > -INFINITY && comp_of(x, j) >= thr) {
         const unsigned bin = bin_of(x);
         atomicAdd(&cnt[bin], 1u);
         if (by_mass) atomicAdd(&mass[bin], weight(x));
       }
-    }
+    });
     __syncthreads();
     locate(by_mass, want, frac, 0, 0, &goal);
     const unsigned bin = s_bin;
     u64 base_c = s_base_c, base_m = s_base_m;
     if (s_bin_n <= LIST) {
-      for (int j = j0 + lane; j < j1; j += 64) {
-        const float x = load_logit(row, j);
+      again([&](float x, int j) {
         if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin) {
           const unsigned at = atomicAdd(&s_n, 1u);
           l_comp[at] = comp_of(x, j);
           l_w[at] = by_mass ? weight(x) : 0;
         }
-      }
+      });
       __syncthreads();
       const int n = (int)s_n;
       for (int i = tid; i < n; i += NT) {
@@ -197,15 +229,14 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
         sh -= nb;
         for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
         __syncthreads();
-        for (int j = j0 + lane; j < j1; j += 64) {
-          const float x = load_logit(row, j);
+        again([&](float x, int j) {
           const unsigned k = key_of(x);
           if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin && (k & pmask) == prefix) {
             const unsigned dig = ~(k >> sh) & ((1u << nb) - 1);            // falling values
             atomicAdd(&cnt[dig], 1u);
             if (by_mass) atomicAdd(&mass[dig], weight(x));
           }
-        }
+        });
         __syncthreads();
         locate(by_mass, want, frac, base_c, base_m, &goal);
         base_c = s_base_c; base_m = s_base_m;
@@ -247,25 +278,120 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     }
     __syncthreads();
   };
+
+  // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
+  // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
+  // wanted ones, and few others.
+  const bool small = VPT > 0 && NT == 256 && V <= 256, few = Kk > 0 && Kk <= 256 && (u64)Kk < nvalid;
+  if (small || few) {
+    if (tid == 0) { s_n = 0; s_bin = NB - 1; }
+    if (!small) {
+      for (int i = tid; i < NB; i += NT) cnt[i] = 0;
+      __syncthreads();
+      if (tmax > -INFINITY) atomicAdd(&cnt[bin_of(tmax)], 1u);
+      __syncthreads();
+      unsigned tc = 0;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) tc += cnt[tid * BPT + i];
+      unsigned ic = tc;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(ic, o); if (lane >= o) ic += y; }
+      if (lane == 63) red_b[w] = ic;
+      __syncthreads();
+      for (int i = 0; i < w; ++i) ic += (unsigned)red_b[i];
+      unsigned ec = ic - tc;
+      if (ec < (unsigned)Kk && ic >= (unsigned)Kk) {
+#pragma unroll
+        for (int i = 0; i < BPT; ++i) {
+          const unsigned nc = cnt[tid * BPT + i];
+          if (ec < (unsigned)Kk && ec + nc >= (unsigned)Kk) s_bin = tid * BPT + i;
+          ec += nc;
+        }
+      }
+    }
+    __syncthreads();
+    const unsigned last = s_bin;
+    each([&](float x, int j) {
+      if (x > -INFINITY && bin_of(x) <= last) {
+        const unsigned at = atomicAdd(&s_n, 1u);
+        if (at < LIST) l_comp[at] = comp_of(x, j);
+      }
+    });
+    __syncthreads();
+    const int n = (int)s_n;
+    if (n <= LIST) {
+      auto value = [&](u64 comp) { return of_key((unsigned)(comp >> 32)); };
+      for (int i = tid; i < n; i += NT) l_w[i] = weight(value(l_comp[i]));
+      __syncthreads();
+      // rank and the weight that lies before; an entry is dropped by setting its weight to 0 (it is not drawn then)
+      constexpr int EPT = LIST / NT;
+      const unsigned want = Kk > 0 ? (unsigned)Kk : ~0u;
+      unsigned rank[EPT];
+      u64 ahead[EPT], sum = 0;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) {
+        const int i = tid + e * NT;
+        rank[e] = ~0u; ahead[e] = 0;
+        if (i < n) {
+          const u64 me = l_comp[i];
+          unsigned r = 0;
+          u64 m = 0;
+          for (int k = 0; k < n; ++k) { const bool up = l_comp[k] > me; r += up; m += up ? l_w[k] : 0; }
+          rank[e] = r; ahead[e] = m;
+          if (r < want) sum += l_w[i];
+        }
+      }
+      sum = wave_sum_u64(sum);
+      if (lane == 0) red_a[w] = sum;
+      __syncthreads();
+      u64 all = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) all += red_a[i];
+      const double goal = fmax((double)P, 0.0) * (double)all;
+      sum = 0;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) {
+        const int i = tid + e * NT;
+        if (i < n) {
+          const u64 me = l_comp[i];
+          const bool keep = rank[e] == 0 || (rank[e] < want && (!(P < 1.f) || (double)ahead[e] < goal) && (value(me) == mx || (double)value(me) >= floor_));
+          if (keep) sum += l_w[i]; else l_w[i] = 0;
+        }
+      }
+      sum = wave_sum_u64(sum);
+      if (lane == 0) red_b[w] = sum;
+      __syncthreads();
+      u64 total = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) total += red_b[i];
+      const double draw = (double)uu * (double)total;
+      for (int i = tid; i < n; i += NT) {
+        const u64 own = l_w[i];
+        if (!own) continue;
+        const unsigned me = (unsigned)l_comp[i];        // ~index: the entries before have a larger one
+        u64 c = 0;
+        for (int k = 0; k < n; ++k) c += (unsigned)l_comp[k] > me ? l_w[k] : 0;
+        if ((double)c <= draw && (double)(c + own) > draw) { a.token[b] = (int)~me; a.logp[b] = logp_of(value(l_comp[i]), total); }
+      }
+      return;
+    }
+    __syncthreads();
+  }
   if (Kk > 0 && (u64)Kk < nvalid) cut(false, (u64)Kk, 0.0);
   if (P < 1.f) cut(true, 0, (double)P);
-  const double floor_ = M > 0.f ? (double)mx + (double)Tm * log((double)M) : -INFINITY;        // w >= m  <=>  x >= max + T ln m
 
   // what is left, in index order
   u64 sum = 0;
   auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
   __syncthreads();
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const float x = load_logit(row, j);
+  again([&](float x, int j) {
     if (kept(x, j)) sum += weight(x);
-  }
+  });
   sum = wave_sum_u64(sum);
   if (lane == 0) red_a[w] = sum;
   __syncthreads();
   u64 total = 0, before = 0;
   for (int i = 0; i < NW; ++i) { if (i < w) before += red_a[i]; total += red_a[i]; }
-  float uu = a.u[b];
-  uu = uu >= 0.f ? fminf(uu, 0.99999994f) : 0.f;
   const double goal = (double)uu * (double)total;
   if (sum && (double)before <= goal && (double)(before + sum) > goal) {       // one wave: the running sums rise
     u64 base = before;
@@ -282,7 +408,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       if (hit) {
         if (lane == __builtin_ctzll(hit)) {
           a.token[b] = j;
-          a.logp[b] = (float)((x == mx ? 0.0 : ((double)x - (double)mx) / (double)Tm) - log(ldexp((double)total, -WBITS)));
+          a.logp[b] = logp_of(x, total);
         }
         break;
       }
@@ -292,8 +418,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
 }
 
 template <typename T> void launch(const SampleArgs& a, int B, hipStream_t st) {
-  if (a.V <= 4096) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024>), dim3(B), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096>), dim3(B), dim3(1024), 0, st, a);
+  if (a.V <= 256) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 1>), dim3(B), dim3(256), 0, st, a);
+  else if (a.V <= 4096) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 16>), dim3(B), dim3(256), 0, st, a);
+  else if (a.V <= 32768) hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 32>), dim3(B), dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 0>), dim3(B), dim3(1024), 0, st, a);
 }
 
 }  // namespace
