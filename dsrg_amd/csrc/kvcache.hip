@@ -316,7 +316,8 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
 }
 
 // MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
-template <int KV, int D, int CT, int NW, bool MIX>
+// UB: 32-token blocks a step, so that a step's keys and values are 8 KB or so each of a wave's loads whatever the type.
+template <int KV, int D, int CT, int NW, bool MIX, int UB>
 __global__ __launch_bounds__(NW * 64) void attention_paged_kernel(const PagedArgs a) {
   typedef typename KvT<KV>::type TS;
   typedef typename std::conditional<KV == DSRG_F32, float, bf16_t>::type TQ;
@@ -370,74 +371,128 @@ __global__ __launch_bounds__(NW * 64) void attention_paged_kernel(const PagedArg
 
   const int32_t* trow = a.table + (long long)b * a.table_ld;
   const int lgB = a.c.lgS - 5, bmask = (1 << lgB) - 1;
-  for (int blk = bbeg + w; blk < bend; blk += NW) {
-    const int page = __builtin_amdgcn_readfirstlane(trow[blk >> lgB]);
-    if (page < 0 || page >= a.c.P) continue;                 // no such page: its tokens are masked
-    const long long ph = (long long)page * H + kh;
-    const long long e0 = (ph * a.c.S + (blk & bmask) * 32) * D;
-    const TS* kb = (const TS*)a.c.k + e0;
-    const TS* vb = (const TS*)a.c.v + e0;
-    using RF = typename std::conditional<F, float4, typename std::conditional<Q8, uint2, uint4>::type>::type;
-    constexpr int E = KvT<KV>::E;
-    RF kr[2][KS], vr[F ? 2 * DT : DT];
+  using RF = typename std::conditional<F, float4, typename std::conditional<Q8, uint2, uint4>::type>::type;
+  constexpr int E = KvT<KV>::E, VN = F ? 2 * DT : DT;
+  RF kr[UB][2][KS], vr[UB][VN];
+  float4 ksc[UB][2], vsc[UB][2];
+  // Where the blocks of one step lie: row0 = the block's first row in the pools (times D: its elements).  A block past the end or on no
+  // page is read from page 0 and counts as masked.
+  struct Step { long long row0[UB]; bool there[UB]; };
+  auto locate = [&](int blk) {
+    Step st;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const RF*>(kb + t * 16 * D + (s * 64 + lane) * E);
-    float4 ksc[2], vsc[2];
-    if constexpr (Q8) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const long long so_ = ph * a.c.S + (blk & bmask) * 32 + 16 * t + 4 * g;
-        ksc[t] = *reinterpret_cast<const float4*>(a.c.ks + so_);
-        vsc[t] = *reinterpret_cast<const float4*>(a.c.vs + so_);
-      }
+    for (int u = 0; u < UB; ++u) {
+      const int at = min(blk + u, bend - 1);
+      const int page = __builtin_amdgcn_readfirstlane(trow[at >> lgB]);
+      st.there[u] = blk + u < bend && page >= 0 && page < a.c.P;
+      st.row0[u] = ((long long)(st.there[u] ? page : 0) * H + kh) * a.c.S + (at & bmask) * 32;
     }
+    return st;
+  };
+  auto load_k = [&](const Step& st) {
 #pragma unroll
-    for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt) vr[dt] = *reinterpret_cast<const RF*>(vb + (dt * 64 + lane) * E);
-    const bool full = blk >= full_lo && blk < full_hi;
-
-    f32x4 s_[CT][2];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) s_[ct][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        if constexpr (F) {
-          const float kf[4] = {kr[t][s].x, kr[t][s].y, kr[t][s].z, kr[t][s].w};
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            const float qq[4] = {qf[ct][s].x, qf[ct][s].y, qf[ct][s].z, qf[ct][s].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s_[ct][t], 0, 0, 0);
-          }
-        } else {
-          bf16x8 kf;
-          if constexpr (Q8) kf = codes_to_bf16(kr[t][s], KV);
-          else kf = __builtin_bit_cast(bf16x8, kr[t][s]);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][s], s_[ct][t], 0, 0, 0);
-        }
-      }
-
-    const int key0 = blk * 32 + 4 * g;
-    float p[CT][8];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float mx = -INFINITY;
+    for (int u = 0; u < UB; ++u) {
+      const TS* kb = (const TS*)a.c.k + st.row0[u] * D;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s_[ct][t][i] * a.sl2;
-          if constexpr (Q8) x *= (&ksc[t].x)[i];
-          if (!full) { const int key = key0 + 16 * t + i; x = key < hi[ct] && key >= lo[ct] ? x : -INFINITY; }
-          p[ct][4 * t + i] = x;
-          mx = fmaxf(mx, x);
+        for (int s = 0; s < KS; ++s) kr[u][t][s] = *reinterpret_cast<const RF*>(kb + t * 16 * D + (s * 64 + lane) * E);
+      if constexpr (Q8) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) ksc[u][t] = *reinterpret_cast<const float4*>(a.c.ks + st.row0[u] + 16 * t + 4 * g);
+      }
+    }
+  };
+  auto load_v = [&](const Step& st) {
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const TS* vb = (const TS*)a.c.v + st.row0[u] * D;
+      if constexpr (Q8) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) vsc[u][t] = *reinterpret_cast<const float4*>(a.c.vs + st.row0[u] + 16 * t + 4 * g);
+      }
+#pragma unroll
+      for (int dt = 0; dt < VN; ++dt) vr[u][dt] = *reinterpret_cast<const RF*>(vb + (dt * 64 + lane) * E);
+    }
+  };
+
+  // The keys of the next step are fetched as soon as this step's are used, the values likewise: a wave always has one of the two in
+  // flight and needs no second set of registers.
+  int blk = bbeg + w * UB;
+  Step cur{}, nxt{};
+  if (blk < bend) { cur = locate(blk); load_k(cur); load_v(cur); }
+  for (; blk < bend; blk += NW * UB) {
+    const bool more = blk + NW * UB < bend;
+    if (more) nxt = locate(blk + NW * UB);
+    f32x4 s_[CT][UB][2];
+#pragma unroll
+    for (int u = 0; u < UB; ++u)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s_[ct][u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if constexpr (F) {
+            const float kf[4] = {kr[u][t][s].x, kr[u][t][s].y, kr[u][t][s].z, kr[u][t][s].w};
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const float qq[4] = {qf[ct][s].x, qf[ct][s].y, qf[ct][s].z, qf[ct][s].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s_[ct][u][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s_[ct][u][t], 0, 0, 0);
+            }
+          } else {
+            bf16x8 kf;
+            if constexpr (Q8) kf = codes_to_bf16(kr[u][t][s], KV);
+            else kf = __builtin_bit_cast(bf16x8, kr[u][t][s]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) s_[ct][u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ct][s], s_[ct][u][t], 0, 0, 0);
+          }
         }
+      }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int u = 0; u < UB; ++u)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_[ct][u][t][i] *= (&ksc[u][t].x)[i];
+    }
+    if (more) load_k(nxt);
+
+    bool full = blk >= full_lo && blk + UB <= full_hi;
+#pragma unroll
+    for (int u = 0; u < UB; ++u) full = full && cur.there[u];
+    const int key0 = blk * 32 + 4 * g;
+    unsigned vis[CT];                      // MIX: a bit per score of the lane
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      vis[ct] = 0;
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < UB; ++u)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + 32 * u + 16 * t + i;
+              const bool in = cur.there[u] && key < hi[ct] && key >= lo[ct];
+              s_[ct][u][t][i] = in ? s_[ct][u][t][i] * a.sl2 : -INFINITY;
+              if (MIX) vis[ct] |= in ? 1u << (8 * u + 4 * t + i) : 0u;
+            }
+      } else {
+#pragma unroll
+        for (int u = 0; u < UB; ++u)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s_[ct][u][t] *= a.sl2;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < UB; ++u)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s_[ct][u][t][0], s_[ct][u][t][1]), fmaxf(s_[ct][u][t][2], s_[ct][u][t][3])));
       const float mn = fmaxf(m[ct], col_max(mx));
       if (__any(mn > m[ct])) {
         const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mn);
@@ -447,102 +502,117 @@ __global__ __launch_bounds__(NW * 64) void attention_paged_kernel(const PagedArg
         m[ct] = mn;
       }
       const float mb = m[ct] == -INFINITY ? 0.f : m[ct];
-      float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { p[ct][j] = __builtin_amdgcn_exp2f(p[ct][j] - mb); sum += p[ct][j]; }
-      l[ct] += sum;
-      if constexpr (Q8) {
+      for (int u = 0; u < UB; ++u)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[ct][4 * t + i] = (full || p[ct][4 * t + i] != 0.f) ? p[ct][4 * t + i] * (&vsc[t].x)[i] : 0.f;
-      }
-    }
-
-    // Tokens of a block that not every column sees may hold anything, and 0 * NaN is NaN: what no column sees is zeroed here,
-    // what only some columns see is looked at below.
-    if (!full) {
-      const int h_all = len, l_all = lo_all;
+          for (int i = 0; i < 4; ++i) s_[ct][u][t][i] = __builtin_amdgcn_exp2f(s_[ct][u][t][i] - mb);
+          l[ct] += (s_[ct][u][t][0] + s_[ct][u][t][1]) + (s_[ct][u][t][2] + s_[ct][u][t][3]);
+          if constexpr (Q8) {
 #pragma unroll
-      for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt)
-#pragma unroll
-        for (int j = 0; j < (F ? 4 : 8); ++j) {
-          const int key = key0 + (F ? 16 * (dt / DT) + j : 16 * (j >> 2) + (j & 3));
-          const bool in = key < h_all && key >= l_all;
-          if constexpr (F) (&vr[dt].x)[j] = in ? (&vr[dt].x)[j] : 0.f;
-          else if constexpr (Q8) { unsigned& u = j < 4 ? vr[dt].x : vr[dt].y; u = in ? u : u & ~(0xffu << (8 * (j & 3))); }
-          else { unsigned& u = (&vr[dt].x)[j >> 1]; u = in ? u : u & (j & 1 ? 0x0000ffffu : 0xffff0000u); }
+            for (int i = 0; i < 4; ++i) s_[ct][u][t][i] = (full || s_[ct][u][t][i] != 0.f) ? s_[ct][u][t][i] * (&vsc[u][t].x)[i] : 0.f;
+          }
         }
     }
-    bool each = false;
-    if constexpr (MIX && !Q8) {
-      // (8-bit codes of a written row are finite, and the scale above is only taken where the token is seen)
-      if (!full) {
-        bool bad = false;
+
+    // Tokens that not every column sees may hold anything, and 0 * NaN is NaN: what no column sees is zeroed here, what only some
+    // columns see is looked at below (8-bit codes of a written row are finite, and its scale is only taken where it is seen).
+    bool odd = false;
+    if (!full) {
 #pragma unroll
-        for (int dt = 0; dt < (F ? 2 * DT : DT); ++dt)
+      for (int u = 0; u < UB; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (F) bad = bad || !(fabsf((&vr[dt].x)[j]) <= 3.4028235e38f);
-            else { const unsigned u = (&vr[dt].x)[j]; bad = bad || (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; }
-          }
-        each = __any(bad);
-      }
-      if (each) {                       // a value that is not finite in a block that only some columns see: column by column
+        for (int dt = 0; dt < VN; ++dt)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll 1
-          for (int col = 0; col < 16; ++col) {
-            const int ch = __shfl(hi[ct], col), cl = __shfl(lo[ct], col);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              f32x4 r = o[ct][dt];
-              if constexpr (F) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 16 * t + i;
-                    r = __builtin_amdgcn_mfma_f32_16x16x4f32(key >= cl && key < ch ? (&vr[t * DT + dt].x)[i] : 0.f, p[ct][4 * t + i], r, 0, 0, 0);
-                  }
-              } else {
-                bf16x8 pf, vf = __builtin_bit_cast(bf16x8, vr[dt]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const int key = key0 + 16 * (j >> 2) + (j & 3);
-                  pf[j] = (__bf16)p[ct][j];
-                  vf[j] = key >= cl && key < ch ? vf[j] : (__bf16)0.f;
-                }
-                r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, r, 0, 0, 0);
-              }
-              if (c16 == col) o[ct][dt] = r;
+          for (int j = 0; j < E; ++j) {
+            const int key = key0 + 32 * u + (F ? 16 * (dt / DT) + j : 16 * (j >> 2) + (j & 3));
+            const bool in = cur.there[u] && key < len && key >= lo_all;
+            if constexpr (F) {
+              float& x = (&vr[u][dt].x)[j];
+              x = in ? x : 0.f;
+              if (MIX) odd = odd || !(fabsf(x) <= 3.4028235e38f);
+            } else if constexpr (Q8) {
+              unsigned& x = j < 4 ? vr[u][dt].x : vr[u][dt].y;
+              x = in ? x : x & ~(0xffu << (8 * (j & 3)));
+            } else {
+              unsigned& x = (&vr[u][dt].x)[j >> 1];
+              const unsigned half = j & 1 ? 0xffff0000u : 0x0000ffffu;
+              x = in ? x : x & ~half;
+              if (MIX) odd = odd || (x & half & 0x7f807f80u) == (half & 0x7f807f80u);
             }
+          }
+    }
+    if constexpr (MIX && !Q8) {
+      if (__any(odd)) {
+        // An infinity or NaN among the values: it leaves V for 0, and three products of 0 / 1 matrices say which columns see a +inf, a -inf or
+        // a NaN of a dim, which is what then goes into the sum.
+#pragma unroll
+        for (int u = 0; u < UB; ++u)
+#pragma unroll
+          for (int dt = 0; dt < VN; ++dt) {
+            float x[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              if constexpr (F) x[j] = (&vr[u][dt].x)[j];
+              else { const unsigned v = (&vr[u][dt].x)[j >> 1]; x[j] = __uint_as_float(j & 1 ? v & 0xffff0000u : v << 16); }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+              for (int kind = 0; kind < 3; ++kind) {
+                f32x4 r = {0.f, 0.f, 0.f, 0.f};
+                auto flag = [&](int j) { return (kind == 0 ? x[j] == INFINITY : kind == 1 ? x[j] == -INFINITY : x[j] != x[j]) ? 1.f : 0.f; };
+                if constexpr (F) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    r = __builtin_amdgcn_mfma_f32_16x16x4f32(flag(j), (float)(vis[ct] >> (8 * u + 4 * (dt / DT) + j) & 1), r, 0, 0, 0);
+                } else {
+                  bf16x8 fa, fb;
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) { fa[j] = (__bf16)flag(j); fb[j] = (__bf16)(float)(vis[ct] >> (8 * u + j) & 1); }
+                  r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb, r, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[ct][dt % DT][i] += r[i] > 0.f ? (kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("")) : 0.f;
+              }
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              if (!(fabsf(x[j]) <= 3.4028235e38f)) {
+                if constexpr (F) (&vr[u][dt].x)[j] = 0.f;
+                else (&vr[u][dt].x)[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+              }
           }
       }
     }
-    if (!each)
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
+    for (int u = 0; u < UB; ++u) {
       if constexpr (F) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32((&vr[t * DT + dt].x)[i], p[ct][4 * t + i], o[ct][dt], 0, 0, 0);
-      } else {
-        bf16x8 pf;
+            for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pf[j] = (__bf16)p[ct][j];
+              for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32((&vr[u][t * DT + dt].x)[i], s_[ct][u][t][i], o[ct][dt], 0, 0, 0);
+      } else {
+        bf16x8 pf[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pf[ct][j] = (__bf16)s_[ct][u][j >> 2][j & 3];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           bf16x8 vf;
-          if constexpr (Q8) vf = codes_to_bf16(vr[dt], KV);
-          else vf = __builtin_bit_cast(bf16x8, vr[dt]);
-          o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[ct][dt], 0, 0, 0);
+          if constexpr (Q8) vf = codes_to_bf16(vr[u][dt], KV);
+          else vf = __builtin_bit_cast(bf16x8, vr[u][dt]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct], o[ct][dt], 0, 0, 0);
         }
       }
     }
+    if (more) { load_v(nxt); cur = nxt; }
   }
 
   // join the waves, one 16-column tile at a time
@@ -604,16 +674,26 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
   float L = 0.f, O[D / 64];
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) O[j] = 0.f;
-  if (M != -INFINITY)
-    for (int s = 0; s < ns; ++s) {
-      const float2 v = ml[s];
-      const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
-      if (f != 0.f) {
-        L += f * v.y;
+  for (int s0 = 0; s0 < ns; s0 += 64) {
+    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing); then 8 splits' partial sums at a time
+    const float2 v = s0 + lane < ns ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+    const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
+    L += wave_sum(f == 0.f ? 0.f : f * v.y);
+    const int cnt = min(64, ns - s0);
+    for (int s = 0; s < cnt; s += 8) {
+      float p[8][D / 64];
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) O[j] += f * a.ws_o[(row * a.nsplit + s) * D + lane + 64 * j];
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) p[t][j] = a.ws_o[(row * a.nsplit + s0 + min(s + t, cnt - 1)) * D + lane + 64 * j];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float ft = s + t < cnt ? lane_f32(f, s + t) : 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) O[j] += ft == 0.f ? 0.f : ft * p[t][j];
       }
     }
+  }
   const int i = n / a.G, h = kh * a.G + n - i * a.G;
   const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
   TQ* op = (TQ*)a.o + b * a.o_bs + (long long)i * a.o_rs + (long long)h * D;
@@ -786,10 +866,11 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
-    if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true>), grid, block, 0, st, a);
-    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true>), grid, block, 0, st, a);
-    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false>), grid, block, 0, st, a);
+    constexpr int UB = D * KvT<KV>::SZ <= 128 ? 2 : 1;
+    if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true, UB>), grid, block, 0, st, a);
+    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true, UB>), grid, block, 0, st, a);
+    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false, UB>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false, UB>), grid, block, 0, st, a);
   }))
   DSRG_LAUNCH_CHECK("dsrg_attention_paged");
   if (s.nsplit > 1) {

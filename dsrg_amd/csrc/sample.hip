@@ -34,6 +34,14 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ u64 comp_of(float x, int j) { return ((u64)key_of(x) << 32) | (unsigned)~j; }
 
+__constant__ const double EXP2_32[32] = {      // 2^(k / 32)
+    1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543,
+    1.6457554781539649, 1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424,
+    1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+
 // 2^(t32 / 32) in WBITS-bit fixed point for t32 <= 0: 2^(n/32) from a table, the rest as e^y, |y| <= ln2 / 64, by its series (the
 // first term left out is y^5 / 120 < 1.3e-12 of the weight).  Adding 2^(52 - WBITS) leaves the rounded fixed-point number in the mantissa.
 __device__ __forceinline__ u64 fixed_exp2(double t32, const double* tab) {
@@ -66,9 +74,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   constexpr int NW = NT / 64, BPT = NB / NT;            // bins per thread
   __shared__ u64 mass[NB];
   __shared__ unsigned cnt[NB];
-  __shared__ u64 l_comp[LIST], l_w[LIST];
+  __shared__ ulonglong2 list[LIST];                     // (comp, weight)
   __shared__ double tab[32];
   __shared__ u64 red_a[NW], red_b[NW];
+  __shared__ float s_max[NW], s_valid[NW];
   __shared__ u64 s_thr, s_base_m, s_base_c, s_bin_m;
   __shared__ unsigned s_bin, s_n, s_bin_n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
@@ -76,7 +85,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
   const int Kk = a.topk ? a.topk[b] : a.topk0;
   const float u_raw = a.u[b], uu = u_raw >= 0.f ? fminf(u_raw, 0.99999994f) : 0.f;
-  if (tid < 32) tab[tid] = exp2(tid / 32.0);
+  if (tid < 32) tab[tid] = EXP2_32[tid];
   // wave w's part of the row: index order is (wave, step, lane)
   const int seg = (V + NW * 64 - 1) / (NW * 64) * 64, j0 = min(V, w * seg), j1 = min(V, j0 + seg);
 
@@ -104,34 +113,30 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     } else again(f);
   };
 
-  // largest value, lowest index first, and how many entries can be drawn at all
+  // largest value, and how many entries can be drawn at all
   float tmax = -INFINITY;
-  int tj = 0;
   unsigned valid = 0;
-  each([&](float x, int j) {
+  each([&](float x, int) {
     valid += x > -INFINITY;
-    if (x > tmax) { tmax = x; tj = j; }                 // (a thread's indices rise)
+    tmax = fmaxf(tmax, x);
   });
-  u64 best = tmax > -INFINITY ? comp_of(tmax, tj) : 0;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const u64 c = __shfl_xor(best, o);
-    best = c > best ? c : best;
-    valid += __shfl_xor(valid, o);
-  }
-  if (lane == 0) { red_a[w] = best; red_b[w] = valid; }
+  const float wmax = wave_max(tmax), wvalid = wave_sum((float)valid);
+  if (lane == 0) { s_max[w] = wmax; s_valid[w] = wvalid; }
   __syncthreads();
-  best = 0;
-  u64 nvalid = 0;
+  float mx = -INFINITY, fvalid = 0.f;                   // (counts up to 2^19: exact)
 #pragma unroll
-  for (int i = 0; i < NW; ++i) { best = red_a[i] > best ? red_a[i] : best; nvalid += red_b[i]; }
+  for (int i = 0; i < NW; ++i) { mx = fmaxf(mx, s_max[i]); fvalid += s_valid[i]; }
+  const int nvalid = (int)fvalid;
   if (nvalid == 0) {                                    // nothing to draw from
     if (tid == 0) { a.token[b] = -1; a.logp[b] = -INFINITY; }
     return;
   }
-  const float mx = of_key((unsigned)(best >> 32));
-  if (!(Tm > 0.f)) {                                    // greedy
-    if (tid == 0) { a.token[b] = (int)~(unsigned)best; a.logp[b] = 0.f; }
+  if (!(Tm > 0.f)) {                                    // greedy: the lowest index of the largest value
+    if (tid == 0) s_n = 0x7fffffff;
+    __syncthreads();
+    each([&](float x, int j) { if (x == mx) atomicMin(&s_n, (unsigned)j); });
+    __syncthreads();
+    if (tid == 0) { a.token[b] = (int)s_n; a.logp[b] = 0.f; }
     return;
   }
   const double c2 = 32 * 1.44269504088896340736 / (double)Tm;
@@ -205,17 +210,20 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       again([&](float x, int j) {
         if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin) {
           const unsigned at = atomicAdd(&s_n, 1u);
-          l_comp[at] = comp_of(x, j);
-          l_w[at] = by_mass ? weight(x) : 0;
+          list[at] = make_ulonglong2(comp_of(x, j), by_mass ? weight(x) : 0);
         }
       });
       __syncthreads();
       const int n = (int)s_n;
       for (int i = tid; i < n; i += NT) {
-        const u64 me = l_comp[i];
+        const u64 me = list[i].x;
         u64 c = base_c, m = base_m;
-        for (int k = 0; k < n; ++k)
-          if (l_comp[k] > me) { ++c; m += l_w[k]; }
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          const ulonglong2 o = list[k];
+          c += o.x > me;
+          m += o.x > me ? o.y : 0;
+        }
         if (by_mass ? (double)m < goal || c == 0 : c < want) atomicMin(&s_thr, me);
       }
       __syncthreads();
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
   // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
   // wanted ones, and few others.
-  const bool small = VPT > 0 && NT == 256 && V <= 256, few = Kk > 0 && Kk <= 256 && (u64)Kk < nvalid;
+  const bool small = VPT > 0 && NT == 256 && V <= 256, few = Kk > 0 && Kk <= 256 && Kk < nvalid;
   if (small || few) {
     if (tid == 0) { s_n = 0; s_bin = NB - 1; }
     if (!small) {
@@ -314,14 +322,15 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     each([&](float x, int j) {
       if (x > -INFINITY && bin_of(x) <= last) {
         const unsigned at = atomicAdd(&s_n, 1u);
-        if (at < LIST) l_comp[at] = comp_of(x, j);
+        if (at < LIST) list[at] = make_ulonglong2(comp_of(x, j), weight(x));
       }
     });
     __syncthreads();
     const int n = (int)s_n;
     if (n <= LIST) {
       auto value = [&](u64 comp) { return of_key((unsigned)(comp >> 32)); };
-      for (int i = tid; i < n; i += NT) l_w[i] = weight(value(l_comp[i]));
+      const int n8 = min((n + 7) & ~7, LIST);           // (up to a multiple of 8 with entries that are behind every other)
+      for (int i = n + tid; i < n8; i += NT) list[i] = make_ulonglong2(0, 0);
       __syncthreads();
       // rank and the weight that lies before; an entry is dropped by setting its weight to 0 (it is not drawn then)
       constexpr int EPT = LIST / NT;
@@ -333,12 +342,18 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
         const int i = tid + e * NT;
         rank[e] = ~0u; ahead[e] = 0;
         if (i < n) {
-          const u64 me = l_comp[i];
+          const ulonglong2 me = list[i];
           unsigned r = 0;
           u64 m = 0;
-          for (int k = 0; k < n; ++k) { const bool up = l_comp[k] > me; r += up; m += up ? l_w[k] : 0; }
+          for (int k = 0; k < n8; k += 8) {
+            ulonglong2 o[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) o[t] = list[k + t];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) { const bool up = o[t].x > me.x; r += up; m += up ? o[t].y : 0; }
+          }
           rank[e] = r; ahead[e] = m;
-          if (r < want) sum += l_w[i];
+          if (r < want) sum += me.y;
         }
       }
       sum = wave_sum_u64(sum);
@@ -353,9 +368,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       for (int e = 0; e < EPT; ++e) {
         const int i = tid + e * NT;
         if (i < n) {
-          const u64 me = l_comp[i];
-          const bool keep = rank[e] == 0 || (rank[e] < want && (!(P < 1.f) || (double)ahead[e] < goal) && (value(me) == mx || (double)value(me) >= floor_));
-          if (keep) sum += l_w[i]; else l_w[i] = 0;
+          const ulonglong2 me = list[i];
+          const float x = value(me.x);
+          const bool keep = rank[e] == 0 || (rank[e] < want && (!(P < 1.f) || (double)ahead[e] < goal) && (x == mx || (double)x >= floor_));
+          if (keep) sum += me.y; else list[i].y = 0;
         }
       }
       sum = wave_sum_u64(sum);
@@ -366,18 +382,24 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       for (int i = 0; i < NW; ++i) total += red_b[i];
       const double draw = (double)uu * (double)total;
       for (int i = tid; i < n; i += NT) {
-        const u64 own = l_w[i];
-        if (!own) continue;
-        const unsigned me = (unsigned)l_comp[i];        // ~index: the entries before have a larger one
+        const ulonglong2 own = list[i];
+        if (!own.y) continue;
+        const unsigned me = (unsigned)own.x;            // ~index: the entries before have a larger one
         u64 c = 0;
-        for (int k = 0; k < n; ++k) c += (unsigned)l_comp[k] > me ? l_w[k] : 0;
-        if ((double)c <= draw && (double)(c + own) > draw) { a.token[b] = (int)~me; a.logp[b] = logp_of(value(l_comp[i]), total); }
+        for (int k = 0; k < n8; k += 8) {
+          ulonglong2 o[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) o[t] = list[k + t];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) c += (unsigned)o[t].x > me ? o[t].y : 0;
+        }
+        if ((double)c <= draw && (double)(c + own.y) > draw) { a.token[b] = (int)~me; a.logp[b] = logp_of(value(own.x), total); }
       }
       return;
     }
     __syncthreads();
   }
-  if (Kk > 0 && (u64)Kk < nvalid) cut(false, (u64)Kk, 0.0);
+  if (Kk > 0 && Kk < nvalid) cut(false, (u64)Kk, 0.0);
   if (P < 1.f) cut(true, 0, (double)P);
 
   // what is left, in index order
