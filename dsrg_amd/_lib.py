@@ -185,3 +185,27 @@ def load():
 def check(rc, what):
     if rc != 0:
         raise DsrgHipError('%s failed (%d): %s' % (what, rc, load().dsrg_last_error().decode()))
+
+
+BIND_PATH = os.path.join(_HERE, 'csrc', '_dsrg_bind.so')
+_bind = None
+
+
+def load_bind():
+    """The CPython module of csrc/bind.cpp (checks, output tensors and the C-ABI call of the serving operators in one native function each),
+    with the loaded library's entry points.  Raises if absent."""
+    global _bind
+    if _bind is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries first)
+        lib = load()
+        if not os.path.exists(BIND_PATH):
+            raise DsrgHipError('%s not found: build it with `python -m dsrg_amd.build`' % BIND_PATH)
+        loader = importlib.machinery.ExtensionFileLoader('_dsrg_bind', BIND_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location('_dsrg_bind', BIND_PATH, loader=loader))
+        loader.exec_module(module)
+        module.init(DsrgHipError, *[C.cast(getattr(lib, 'dsrg_' + n), C.c_void_p).value for n in
+                                    ('last_error', 'kv_append', 'kv_read', 'attention_paged_workspace', 'attention_paged', 'sample_rows')])
+        _bind = module
+    return _bind

@@ -1,4 +1,4 @@
-"""Build libdsrg_hip.so for gfx950 with hipcc (cross-compiles without a GPU).
+"""Build libdsrg_hip.so for gfx950 with hipcc (cross-compiles without a GPU) and the host module _dsrg_bind.so.
 
     python -m dsrg_amd.build [--force]
 """
@@ -9,6 +9,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(CSRC, 'libdsrg_hip.so')
+BIND = os.path.join(CSRC, '_dsrg_bind.so')          # CPython module (bind.cpp): native host side of the serving operators
 SOURCES = ['gemm.hip', 'rowops.hip', 'attention.hip', 'train.hip', 'train_rows.hip', 'graphmap.hip', 'optim.hip', 'kvcache.hip', 'sample.hip']
 HEADERS = ['common.h', os.path.join('..', '..', 'include', 'dsrg_hip.h')]
 
@@ -21,7 +22,20 @@ def _stale():
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
+    if not os.path.exists(BIND) or os.path.getmtime(os.path.join(CSRC, 'bind.cpp')) > os.path.getmtime(BIND):
+        return True
     return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+
+
+def _bind_command():
+    """host code only, against this interpreter's and this torch's headers (HIP's headers want to be told the platform by a compiler that
+    is not hipcc)"""
+    import sysconfig
+    import torch
+    t = os.path.dirname(torch.__file__)
+    inc = [os.path.join(t, 'include'), os.path.join(t, 'include', 'torch', 'csrc', 'api', 'include'), '/opt/rocm/include', sysconfig.get_paths()['include']]
+    return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', *['-isystem' + i for i in inc],
+            os.path.join(CSRC, 'bind.cpp'), '-o', BIND, '-L' + os.path.join(t, 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10', '-lc10_hip']
 
 
 def build(force=False, verbose=True):
@@ -37,9 +51,13 @@ def build(force=False, verbose=True):
             print(' '.join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd)))
         objs.append(obj)
+    cmd = _bind_command()
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    procs.append(('bind.cpp', subprocess.Popen(cmd)))
     for src, p in procs:
         if p.wait() != 0:
-            raise RuntimeError('hipcc failed on %s' % src)
+            raise RuntimeError('the compiler failed on %s' % src)
     cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs
     if verbose:
         print(' '.join(cmd), flush=True)

@@ -11,6 +11,7 @@
 // group): 4-element chunks, K [S/16][D/4][16][4], V [S/16][D/16][4 g][16][4 i].
 #include "common.h"
 #include <math.h>
+#include <algorithm>
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -317,8 +318,10 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
 
 // MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
 // UB: 32-token blocks a step, so that a step's keys and values are 8 KB or so each of a wave's loads whatever the type.
+// Workgroups of four waves that a CU holds: bounded by the registers of O, of the step's keys and values and of the queries.
+constexpr int resident(int kv, int D, int CT) { return D == 64 ? (CT == 1 ? 4 : 3) - (kv == DSRG_F32) : kv == DSRG_F32 ? 1 : 2; }
 template <int KV, int D, int CT, int NW, bool MIX, int UB>
-__global__ __launch_bounds__(NW * 64) void attention_paged_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_kernel(const PagedArgs a) {
   typedef typename KvT<KV>::type TS;
   typedef typename std::conditional<KV == DSRG_F32, float, bf16_t>::type TQ;
   constexpr bool F = KV == DSRG_F32, Q8 = KvT<KV>::SZ == 1;
@@ -724,17 +727,16 @@ int check_table(const char* who, const int32_t* table, int ld, int width, int S,
 bool rows16(const void* p, long long bs, long long rs, int size) { return (uintptr_t)p % 16 == 0 && bs * size % 16 == 0 && rs * size % 16 == 0; }
 
 struct Split { int nsplit, bps; };
-// Workgroups that the chip should get (256 CUs), and the fewest 32-token blocks that a workgroup should have.
-Split plan_split(int B, int H, int cgs, long long max_tokens) {
-  const long long blocks = (max_tokens + 31) / 32, have = (long long)B * H * cgs;
-  long long ns = (1024 + have - 1) / have;
-  if (ns > (blocks + 7) / 8) ns = (blocks + 7) / 8;
-  if (ns < 1) ns = 1;
-  if (ns > 512) ns = 512;
-  long long bps = (blocks + ns - 1) / ns;
-  if (bps < 1) bps = 1;
-  ns = (blocks + bps - 1) / bps;
-  return Split{(int)(ns < 1 ? 1 : ns), (int)bps};
+// The tokens of a sequence are split so that the workgroups fill the chip's places (256 CUs) about once: fewer leave CUs idle, more than fit
+// wait for a second round and have to be joined all the same.  A workgroup gets 256 tokens at least (below, the join costs more than it
+// saves), and 16384 at most, so that one long sequence among short ones does not run alone for long.
+Split plan_split(int kv, int D, int ct, int B, int H, int cgs, long long max_tokens) {
+  const long long blocks = (max_tokens + 31) / 32, have = (long long)B * H * cgs, places = 256ll * resident(kv, D, ct);
+  long long ns = (2 * places + have) / (2 * have);
+  ns = std::min(std::max(ns, (blocks + 511) / 512), (blocks + 7) / 8);
+  ns = std::min(std::max(ns, 1ll), 1024ll);
+  const long long bps = std::max((blocks + ns - 1) / ns, 1ll);
+  return Split{(int)std::max((blocks + bps - 1) / bps, 1ll), (int)bps};
 }
 long long seen_tokens(int width, int S, int Nq, int window) {
   const long long cap = (long long)width * S;
@@ -830,7 +832,7 @@ extern "C" int64_t dsrg_attention_paged_workspace(const dsrg_kv_cache_t* cache, 
   const long long NC = (long long)Nq * (nh / p.H);
   DSRG_CHECK(NC <= (1 << 20), "dsrg_attention_paged_workspace: %lld query rows per key / value head", NC);
   const int ct = col_tiles((int)NC), cgs = (int)((NC + 16 * ct - 1) / (16 * ct));
-  const Split s = plan_split(B, p.H, cgs, seen_tokens(width, p.S, Nq, window));
+  const Split s = plan_split(cache->dtype, cache->head_dim, ct, B, p.H, cgs, seen_tokens(width, p.S, Nq, window));
   return s.nsplit > 1 ? (int64_t)B * p.H * NC * s.nsplit * (cache->head_dim * 4 + 8) : 0;
 }
 
@@ -856,7 +858,7 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   a.NC = Nq * a.G;
   const int ct = col_tiles(a.NC), cgs = (a.NC + 16 * ct - 1) / (16 * ct);
   DSRG_CHECK((long long)a.c.H * cgs <= 65535, "dsrg_attention_paged: %d query rows per key / value head", a.NC);
-  const Split s = plan_split(B, a.c.H, cgs, seen_tokens(width, a.c.S, Nq, window));
+  const Split s = plan_split(cache->dtype, D_, ct, B, a.c.H, cgs, seen_tokens(width, a.c.S, Nq, window));
   a.q = q; a.o = o; a.lse = lse; a.q_bs = q_bs; a.o_bs = o_bs; a.q_rs = q_rs; a.o_rs = o_rs;
   a.table = table; a.lens = lens; a.table_ld = table_ld; a.width = width; a.B = B; a.nh = nh; a.Nq = Nq;
   a.causal = causal != 0; a.window = window; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
@@ -866,7 +868,7 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
-    constexpr int UB = D * KvT<KV>::SZ <= 128 ? 2 : 1;
+    constexpr int UB = D == 128 && KvT<KV>::SZ == 1 ? 2 : 1;
     if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true, UB>), grid, block, 0, st, a);
     else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true, UB>), grid, block, 0, st, a);
     else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false, UB>), grid, block, 0, st, a);

@@ -815,13 +815,7 @@ def action_tail(logits, targets=None, u=None, ignore_index=-100, want_grad=False
     return out
 
 
-_PARAM = {'temperature': (torch.float32, 'fp32'), 'top_k': (torch.int32, 'int32'), 'top_p': (torch.float32, 'fp32'), 'min_p': (torch.float32, 'fp32')}
-
-
-def _elsewhere(dev):
-    """True where tensors lie on another device than the current one (the caller enters that device and calls again)."""
-    return dev.index is not None and dev.index != torch.cuda.current_device()
-
+# ---- serving operators: the checks and the call are native code (csrc/bind.cpp) ----------------------------------------------
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One entry of each row of logits [B,V] (fp32 / bf16, rows contiguous, -inf and NaN = not a candidate), drawn with the given
@@ -829,37 +823,10 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     and min_p (<= 0: off) are numbers or tensors [B] (fp32, top_k int32).  The cuts apply in that order, each to what the one before left; equal
     values rank by index; the draw runs over what is left in index order (dsrg_sample_rows).  A row without a candidate: token -1, logp
     -inf."""
-    lib = _lib.load()
-    _dev(logits)
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise _lib.DsrgHipError('sample_rows: logits must be [B,V] with contiguous rows')
-    dt = _dt(logits)
-    B, V = logits.shape
-    dev = logits.device
-    if u.dtype != torch.float32 or u.shape != (B,) or not u.is_contiguous() or u.device != dev:
-        raise _lib.DsrgHipError('sample_rows: u must be contiguous fp32 [B] beside the logits')
-    ptr, num = [], []
-    for name, x in (('temperature', temperature), ('top_k', top_k), ('top_p', top_p), ('min_p', min_p)):
-        if isinstance(x, torch.Tensor):
-            want, text = _PARAM[name]
-            if x.dtype != want or x.shape != (B,) or not x.is_contiguous() or x.device != dev:
-                raise _lib.DsrgHipError('sample_rows: %s must be a number or contiguous %s [B] beside the logits' % (name, text))
-            ptr.append(x.data_ptr())
-            num.append(0)
-        else:
-            ptr.append(None)
-            num.append(x)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return sample_rows(logits, u, temperature, top_k, top_p, min_p)
-    token = torch.empty(B, device=dev, dtype=torch.int64)
-    logp = torch.empty(B, device=dev, dtype=torch.float32)
-    _lib.check(lib.dsrg_sample_rows(logits.data_ptr(), logits.stride(0) if B > 1 else V, dt, u.data_ptr(), ptr[0], num[0], ptr[1], int(num[1]), ptr[2], num[2],
-                                    ptr[3], num[3], token.data_ptr(), logp.data_ptr(), B, V, _stream()), 'dsrg_sample_rows')
-    return token, logp
+    return (_lib._bind or _lib.load_bind()).sample_rows(logits, u, temperature, top_k, top_p, min_p)
 
 
-_KV_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
+_KV_DT = (torch.float32, torch.bfloat16, torch.int8, torch.float8_e4m3fn)
 
 
 def kv_pool_shapes(n_pages, page_size, n_kv_heads, head_dim, dtype):
@@ -874,86 +841,16 @@ def kv_pool_shapes(n_pages, page_size, n_kv_heads, head_dim, dtype):
     return (n_pages, n_kv_heads, page_size // 16, head_dim // 8, 16, 8), (n_pages, n_kv_heads, page_size // 32, head_dim // 16, 4, 16, 2, 4)
 
 
-def _kv_cache(what, k_pool, v_pool, k_scale, v_scale):
-    """dsrg_kv_cache_t over the four buffers -> (struct, kv heads, head dim)"""
-    _dev(k_pool)
-    dt = _KV_DT.get(k_pool.dtype)
-    if dt is None or k_pool.dim() != 6:
-        raise _lib.DsrgHipError('%s: k_pool %s %s is no cache (kv_pool_shapes)' % (what, k_pool.dtype, tuple(k_pool.shape)))
-    P, H, S, D = k_pool.shape[0], k_pool.shape[1], k_pool.shape[2] * 16, k_pool.shape[3] * k_pool.shape[5]
-    ks, vs = kv_pool_shapes(P, S, H, D, k_pool.dtype)
-    if k_pool.shape != ks or v_pool.shape != vs or v_pool.dtype != k_pool.dtype or not k_pool.is_contiguous() or not v_pool.is_contiguous() or v_pool.device != k_pool.device:
-        raise _lib.DsrgHipError('%s: pools must be contiguous %s and %s of one dtype (got %s, %s)' % (what, ks, vs, tuple(k_pool.shape), tuple(v_pool.shape)))
-    if dt >= _lib.I8:
-        for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.float32 or s.shape != (P, H, S) or not s.is_contiguous() or s.device != k_pool.device:
-                raise _lib.DsrgHipError('%s: an 8-bit cache needs k_scale and v_scale, contiguous fp32 [pages, kv heads, page size]' % what)
-    elif k_scale is not None or v_scale is not None:
-        raise _lib.DsrgHipError('%s: only 8-bit caches have scales' % what)
-    return _lib.KvCache(k_pool.data_ptr(), v_pool.data_ptr(), _p(k_scale), _p(v_scale), P, S, H, D, dt, 0), H, D
-
-
-def _kv_table(what, table, dev, B):
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1) or table.device != dev:
-        raise _lib.DsrgHipError('%s: the page table must be int32 [B, pages] with contiguous rows beside the cache' % what)
-    return table.data_ptr(), max(table.stride(0), table.shape[1]) if B == 1 else table.stride(0), table.shape[1]
-
-
-def _kv_ints(what, name, x, dev, B):
-    if x.dtype != torch.int32 or x.shape != (B,) or not x.is_contiguous() or x.device != dev:
-        raise _lib.DsrgHipError('%s: %s must be contiguous int32 [B] beside the cache' % (what, name))
-    return x.data_ptr()
-
-
-def _rows16(t):
-    """[B,N,W] as it is if its rows are contiguous and 16-byte aligned, else a copy -> (tensor, batch stride, row stride)"""
-    n = 16 // t.element_size()
-    if (t.stride(2) != 1 and t.shape[2] > 1) or t.data_ptr() % 16 or (t.stride(0) % n and t.shape[0] > 1) or (t.stride(1) % n and t.shape[1] > 1):
-        t = t.clone(memory_format=torch.contiguous_format)
-    W = t.shape[2]
-    rs = t.stride(1) if t.shape[1] > 1 else W
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1] * rs, rs
-
-
 def kv_append(k, v, k_pool, v_pool, table, start, count=None, k_scale=None, v_scale=None):
     """Write rows t < count[b] (None: all T) of k / v [B, T, kv heads * head dim] as tokens start[b] + t of sequence b into a paged cache,
     quantising where its pools are int8 / float8_e4m3fn (dsrg_kv_append).  table int32 [B, pages], start / count int32 [B]."""
-    lib = _lib.load()
-    c, H, D = _kv_cache('kv_append', k_pool, v_pool, k_scale, v_scale)
-    dev = k_pool.device
-    if k.dim() != 3 or k.shape[2] != H * D or v.shape != k.shape or v.dtype != k.dtype or k.device != dev or v.device != dev:
-        raise _lib.DsrgHipError('kv_append: k and v must be [B, T, %d] of one dtype beside the cache (got %s, %s)' % (H * D, tuple(k.shape), tuple(v.shape)))
-    dt = _dt(k)
-    B, T, _ = k.shape
-    tp, ld, width = _kv_table('kv_append', table, dev, B)
-    sp = _kv_ints('kv_append', 'start', start, dev, B)
-    cp = None if count is None else _kv_ints('kv_append', 'count', count, dev, B)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return kv_append(k, v, k_pool, v_pool, table, start, count, k_scale, v_scale)
-    k, kb, kr = _rows16(k)
-    v, vb, vr = _rows16(v)
-    _lib.check(lib.dsrg_kv_append(c, k.data_ptr(), kb, kr, v.data_ptr(), vb, vr, dt, tp, ld, width, sp, cp, B, T, _stream()), 'dsrg_kv_append')
+    (_lib._bind or _lib.load_bind()).kv_append(k, v, k_pool, v_pool, table, start, count, k_scale, v_scale)
 
 
 def kv_read(k_pool, v_pool, table, start, count, n, k_scale=None, v_scale=None, dtype=None):
     """Tokens start[b] + t, t < count[b], of each sequence as dense k, v [B, n, kv heads * head dim] (rows t >= count[b] zero).  dtype: the
     cache's own; float32 or bfloat16 (default) for 8-bit caches."""
-    lib = _lib.load()
-    c, H, D = _kv_cache('kv_read', k_pool, v_pool, k_scale, v_scale)
-    dev, B = k_pool.device, table.shape[0]
-    dtype = dtype or (torch.bfloat16 if c.dtype >= _lib.I8 else k_pool.dtype)
-    dt = _dt(dtype)
-    tp, ld, width = _kv_table('kv_read', table, dev, B)
-    sp, cp = _kv_ints('kv_read', 'start', start, dev, B), _kv_ints('kv_read', 'count', count, dev, B)
-    if n < 0:
-        raise _lib.DsrgHipError('kv_read: n = %d' % n)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return kv_read(k_pool, v_pool, table, start, count, n, k_scale, v_scale, dtype)
-    k, v = (torch.empty(B, n, H * D, device=dev, dtype=dtype) for _ in range(2))
-    _lib.check(lib.dsrg_kv_read(c, k.data_ptr(), n * H * D, H * D, v.data_ptr(), n * H * D, H * D, dt, tp, ld, width, sp, cp, B, n, _stream()), 'dsrg_kv_read')
-    return k, v
+    return (_lib._bind or _lib.load_bind()).kv_read(k_pool, v_pool, table, start, count, n, k_scale, v_scale, dtype)
 
 
 def attention_paged(q, k_pool, v_pool, table, lens, nh, k_scale=None, v_scale=None, scale=None, causal=False, window=0, want_lse=False):
@@ -961,29 +858,7 @@ def attention_paged(q, k_pool, v_pool, table, lens, nh, k_scale=None, v_scale=No
     [B, nh, Nq]); nh is a multiple of the cache's heads.  causal: the Nq rows are the newest tokens (already written), each sees itself
     and what is before it, with window > 0 the last `window` of those.  scale: 1 / sqrt(head dim) by default.  bf16 q, fp32 for an
     fp32 cache.  Rows that see nothing: o = 0, lse = -inf (dsrg_attention_paged)."""
-    lib = _lib.load()
-    c, H, D = _kv_cache('attention_paged', k_pool, v_pool, k_scale, v_scale)
-    dev = k_pool.device
-    if q.dim() != 3 or nh < 1 or nh % H or q.shape[2] != nh * D or q.device != dev:
-        raise _lib.DsrgHipError('attention_paged: q %s is not [B, Nq, nh * %d] with nh = %s a multiple of %d, beside the cache' % (tuple(q.shape), D, nh, H))
-    dt = _dt(q)
-    B, Nq, W = q.shape
-    tp, ld, width = _kv_table('attention_paged', table, dev, B)
-    lp = _kv_ints('attention_paged', 'lens', lens, dev, B)
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return attention_paged(q, k_pool, v_pool, table, lens, nh, k_scale, v_scale, scale, causal, window, want_lse)
-    q, qb, qr = _rows16(q)
-    out = torch.empty(B, Nq, W, device=dev, dtype=q.dtype)
-    lse = torch.empty(B, nh, Nq, device=dev, dtype=torch.float32) if want_lse else None
-    ws, need = None, lib.dsrg_attention_paged_workspace(c, width, B, nh, Nq, int(window))
-    if need < 0:
-        _lib.check(need, 'dsrg_attention_paged_workspace')
-    if need:
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-    _lib.check(lib.dsrg_attention_paged(c, q.data_ptr(), qb, qr, out.data_ptr(), Nq * W, W, _p(lse), tp, ld, width, lp, B, nh, Nq, D ** -0.5 if scale is None else scale,
-                                        int(causal), int(window), _p(ws), need, dt, _stream()), 'dsrg_attention_paged')
-    return (out, lse) if want_lse else out
+    return (_lib._bind or _lib.load_bind()).attention_paged(q, k_pool, v_pool, table, lens, nh, k_scale, v_scale, scale, causal, window, want_lse)
 
 
 def ce_rows(logits, targets, ignore_index=-100):
