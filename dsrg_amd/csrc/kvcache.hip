@@ -320,6 +320,8 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
 // UB: 32-token blocks a step, so that a step's keys and values are 8 KB or so each of a wave's loads whatever the type.
 // Workgroups of four waves that a CU holds: bounded by the registers of O, of the step's keys and values and of the queries.
 constexpr int resident(int kv, int D, int CT) { return D == 64 ? (CT == 1 ? 4 : 3) - (kv == DSRG_F32) : kv == DSRG_F32 ? 1 : 2; }
+// 32-token blocks a step (one 16-column tile; with two the registers do not hold more than one)
+constexpr int step_blocks(int kv, int D) { return D == 128 && (kv == DSRG_I8 || kv == DSRG_E4M3) ? 2 : 1; }
 template <int KV, int D, int CT, int NW, bool MIX, int UB>
 __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_kernel(const PagedArgs a) {
   typedef typename KvT<KV>::type TS;
@@ -868,11 +870,10 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
-    constexpr int UB = D == 128 && KvT<KV>::SZ == 1 ? 2 : 1;
-    if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true, UB>), grid, block, 0, st, a);
-    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true, UB>), grid, block, 0, st, a);
-    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false, UB>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false, UB>), grid, block, 0, st, a);
+        if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true, step_blocks(KV, D)>), grid, block, 0, st, a);
+    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true, 1>), grid, block, 0, st, a);
+    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false, step_blocks(KV, D)>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false, 1>), grid, block, 0, st, a);
   }))
   DSRG_LAUNCH_CHECK("dsrg_attention_paged");
   if (s.nsplit > 1) {

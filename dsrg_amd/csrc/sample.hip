@@ -56,9 +56,35 @@ __device__ __forceinline__ u64 fixed_exp2(double t32, const double* tab) {
   return (u64)__double_as_longlong(ldexp(e * tab[n & 31], n >> 5) + MAGIC) - (u64)__builtin_bit_cast(long long, MAGIC);
 }
 
+template <int CTRL> __device__ __forceinline__ u64 dpp_u64(u64 v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, 0xF, 0xF, true);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, 0xF, 0xF, true);
+  return (u64)hi << 32 | lo;
+}
+// sum over the 16 lanes of a DPP row, in all of them
+__device__ __forceinline__ u64 row_sum_u64(u64 v) {
+  v += dpp_u64<0xB1>(v);
+  v += dpp_u64<0x4E>(v);
+  v += dpp_u64<0x141>(v);
+  return v + dpp_u64<0x140>(v);
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int l) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, l);
+}
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  v = row_sum_u64(v);
+  return (lane_u64(v, 0) + lane_u64(v, 16)) + (lane_u64(v, 32) + lane_u64(v, 48));
+}
+// inclusive running sum over the wave
+__device__ __forceinline__ unsigned wave_scan_u32(unsigned v) {
+#define DSRG_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true)
+  DSRG_STEP(0x111, 0xF);      // row_shr 1, 2, 4, 8: inside the rows of 16
+  DSRG_STEP(0x112, 0xF);
+  DSRG_STEP(0x114, 0xF);
+  DSRG_STEP(0x118, 0xF);
+  DSRG_STEP(0x142, 0xA);      // row_bcast 15: rows 1 and 3 get what rows 0 and 2 end with
+  DSRG_STEP(0x143, 0xC);      // row_bcast 31: rows 2 and 3 get what row 1 ends with
+#undef DSRG_STEP
   return v;
 }
 
@@ -75,6 +101,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   __shared__ u64 mass[NB];
   __shared__ unsigned cnt[NB];
   __shared__ ulonglong2 list[LIST];                     // (comp, weight)
+  u64* const l_ahead = mass;                            // (the short way has no use for the bins' weights)
+  unsigned* const l_rank = cnt;
+  static_assert(NB >= LIST, "one word an entry");
   __shared__ double tab[32];
   __shared__ u64 red_a[NW], red_b[NW];
   __shared__ float s_max[NW], s_valid[NW];
@@ -154,6 +183,27 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   };
   const double floor_ = M > 0.f ? (double)mx + (double)Tm * log((double)M) : -INFINITY;        // w >= m  <=>  x >= max + T ln m
 
+  // For every entry of the list, by the 16 lanes of a DPP row together: how many entries `ahead(other, me)` holds for and what they weigh.
+  auto ranked = [&](int n, auto&& ahead, auto&& f) {
+    const int sub = tid & 15;
+    for (int i0 = 0; i0 < n; i0 += NT / 16) {
+      const int i = i0 + (tid >> 4);
+      const ulonglong2 me = list[min(i, n - 1)];
+      unsigned c = 0;
+      u64 m = 0;
+#pragma unroll 4
+      for (int k = sub; k < n; k += 16) {
+        const ulonglong2 o = list[k];
+        const bool up = ahead(o, me);
+        c += up;
+        m += up ? o.y : 0;
+      }
+      const u64 cs = row_sum_u64(c);
+      m = row_sum_u64(m);
+      if (sub == 0 && i < n) f(i, me, (unsigned)cs, m);
+    }
+  };
+  auto larger = [](const ulonglong2& o, const ulonglong2& me) { return o.x > me.x; };
   // Running count and weight over the bins, behind (c0, m0); the first bin that reaches the goal goes to s_bin, with what lies
   // before it and what it holds.  *goal < 0: it is frac of what all bins weigh.  (Entries so far down that their weight rounds to
   // 0 never reach a goal: the last bin that weighs anything does.)
@@ -215,17 +265,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       });
       __syncthreads();
       const int n = (int)s_n;
-      for (int i = tid; i < n; i += NT) {
-        const u64 me = list[i].x;
-        u64 c = base_c, m = base_m;
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-          const ulonglong2 o = list[k];
-          c += o.x > me;
-          m += o.x > me ? o.y : 0;
-        }
-        if (by_mass ? (double)m < goal || c == 0 : c < want) atomicMin(&s_thr, me);
-      }
+      ranked(n, larger, [&](int, const ulonglong2& me, unsigned c, u64 m) {
+        if (by_mass ? (double)(base_m + m) < goal || base_c + c == 0 : base_c + c < want) atomicMin(&s_thr, me.x);
+      });
       __syncthreads();
       thr = s_thr;
     } else {
@@ -289,73 +331,56 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
 
   // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
   // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
-  // wanted ones, and few others.
-  const bool small = VPT > 0 && NT == 256 && V <= 256, few = Kk > 0 && Kk <= 256 && Kk < nvalid;
+  // wanted ones, and few others.  One bin a thread here (NT / 16 an octave): a bin costs a few more entries, a scan more costs time.
+  const bool small = VPT == 1, few = Kk > 0 && Kk <= 256 && Kk < nvalid;
   if (small || few) {
-    if (tid == 0) { s_n = 0; s_bin = NB - 1; }
+    float edge = 0.f;                                   // the candidates with max - x < edge, or every one
+    bool every = true;
+    if (tid == 0) s_n = 0;
     if (!small) {
-      for (int i = tid; i < NB; i += NT) cnt[i] = 0;
+      constexpr int SN = 23 - (NT == 1024 ? 6 : 4);
+      static_assert(NT == 1024 || NT == 256, "NT / 16 bins an octave");
+      constexpr unsigned lo = 0x3b800000u >> SN;
+      cnt[tid] = 0;
+      if (tid == 0) s_bin = NT;                         // (fewer than k threads have an entry at all: everything)
       __syncthreads();
-      if (tmax > -INFINITY) atomicAdd(&cnt[bin_of(tmax)], 1u);
+      if (tmax > -INFINITY) {
+        const unsigned d = __float_as_uint(mx == tmax ? 0.f : mx - tmax) >> SN;
+        atomicAdd(&cnt[d < lo ? 0u : min(d - lo, (unsigned)NT - 1)], 1u);
+      }
       __syncthreads();
-      unsigned tc = 0;
-#pragma unroll
-      for (int i = 0; i < BPT; ++i) tc += cnt[tid * BPT + i];
-      unsigned ic = tc;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(ic, o); if (lane >= o) ic += y; }
+      const unsigned tc = cnt[tid];
+      unsigned ic = wave_scan_u32(tc);
       if (lane == 63) red_b[w] = ic;
       __syncthreads();
-      for (int i = 0; i < w; ++i) ic += (unsigned)red_b[i];
-      unsigned ec = ic - tc;
-      if (ec < (unsigned)Kk && ic >= (unsigned)Kk) {
 #pragma unroll
-        for (int i = 0; i < BPT; ++i) {
-          const unsigned nc = cnt[tid * BPT + i];
-          if (ec < (unsigned)Kk && ec + nc >= (unsigned)Kk) s_bin = tid * BPT + i;
-          ec += nc;
-        }
-      }
-    }
-    __syncthreads();
-    const unsigned last = s_bin;
+      for (int i = 0; i < NW; ++i) ic += i < w ? (unsigned)red_b[i] : 0u;
+      if (ic >= (unsigned)Kk && ic - tc < (unsigned)Kk) s_bin = tid;
+      __syncthreads();
+      const unsigned last = s_bin;
+      every = last >= NT - 1;
+      if (!every) edge = __uint_as_float((last + lo + 1) << SN);
+    } else __syncthreads();
     each([&](float x, int j) {
-      if (x > -INFINITY && bin_of(x) <= last) {
+      if (every ? x > -INFINITY : x == mx || mx - x < edge) {
         const unsigned at = atomicAdd(&s_n, 1u);
-        if (at < LIST) list[at] = make_ulonglong2(comp_of(x, j), weight(x));
+        if (at < LIST) list[at].x = comp_of(x, j);
       }
     });
     __syncthreads();
     const int n = (int)s_n;
     if (n <= LIST) {
       auto value = [&](u64 comp) { return of_key((unsigned)(comp >> 32)); };
-      const int n8 = min((n + 7) & ~7, LIST);           // (up to a multiple of 8 with entries that are behind every other)
-      for (int i = n + tid; i < n8; i += NT) list[i] = make_ulonglong2(0, 0);
+      for (int i = tid; i < n; i += NT) list[i].y = weight(value(list[i].x));
       __syncthreads();
-      // rank and the weight that lies before; an entry is dropped by setting its weight to 0 (it is not drawn then)
-      constexpr int EPT = LIST / NT;
       const unsigned want = Kk > 0 ? (unsigned)Kk : ~0u;
-      unsigned rank[EPT];
-      u64 ahead[EPT], sum = 0;
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) {
-        const int i = tid + e * NT;
-        rank[e] = ~0u; ahead[e] = 0;
-        if (i < n) {
-          const ulonglong2 me = list[i];
-          unsigned r = 0;
-          u64 m = 0;
-          for (int k = 0; k < n8; k += 8) {
-            ulonglong2 o[8];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) o[t] = list[k + t];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) { const bool up = o[t].x > me.x; r += up; m += up ? o[t].y : 0; }
-          }
-          rank[e] = r; ahead[e] = m;
-          if (r < want) sum += me.y;
-        }
-      }
+      // rank and the weight ahead of every entry; what the first want ones weigh (only top-p asks for it)
+      u64 sum = 0;
+      ranked(n, larger, [&](int i, const ulonglong2& me, unsigned c, u64 m) {
+        l_rank[i] = c;
+        l_ahead[i] = m;
+        if (c < want) sum += me.y;
+      });
       sum = wave_sum_u64(sum);
       if (lane == 0) red_a[w] = sum;
       __syncthreads();
@@ -364,15 +389,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       for (int i = 0; i < NW; ++i) all += red_a[i];
       const double goal = fmax((double)P, 0.0) * (double)all;
       sum = 0;
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) {
-        const int i = tid + e * NT;
-        if (i < n) {
-          const ulonglong2 me = list[i];
-          const float x = value(me.x);
-          const bool keep = rank[e] == 0 || (rank[e] < want && (!(P < 1.f) || (double)ahead[e] < goal) && (x == mx || (double)x >= floor_));
-          if (keep) sum += me.y; else list[i].y = 0;
-        }
+      for (int i = tid; i < n; i += NT) {               // what is not kept loses its weight: it is not drawn then
+        const ulonglong2 me = list[i];
+        const float x = value(me.x);
+        const unsigned rank = l_rank[i];
+        const bool keep = rank == 0 || (rank < want && (!(P < 1.f) || (double)l_ahead[i] < goal) && (x == mx || (double)x >= floor_));
+        if (keep) sum += me.y; else list[i].y = 0;
       }
       sum = wave_sum_u64(sum);
       if (lane == 0) red_b[w] = sum;
@@ -381,20 +403,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
 #pragma unroll
       for (int i = 0; i < NW; ++i) total += red_b[i];
       const double draw = (double)uu * (double)total;
-      for (int i = tid; i < n; i += NT) {
-        const ulonglong2 own = list[i];
-        if (!own.y) continue;
-        const unsigned me = (unsigned)own.x;            // ~index: the entries before have a larger one
-        u64 c = 0;
-        for (int k = 0; k < n8; k += 8) {
-          ulonglong2 o[8];
-#pragma unroll
-          for (int t = 0; t < 8; ++t) o[t] = list[k + t];
-#pragma unroll
-          for (int t = 0; t < 8; ++t) c += (unsigned)o[t].x > me ? o[t].y : 0;
-        }
-        if ((double)c <= draw && (double)(c + own.y) > draw) { a.token[b] = (int)~me; a.logp[b] = logp_of(value(own.x), total); }
-      }
+      // (the low word is ~index: the entries before have a larger one)
+      ranked(n, [](const ulonglong2& o, const ulonglong2& me) { return (unsigned)o.x > (unsigned)me.x; }, [&](int, const ulonglong2& me, unsigned, u64 m) {
+        if (me.y && (double)m <= draw && (double)(m + me.y) > draw) { a.token[b] = (int)~(unsigned)me.x; a.logp[b] = logp_of(value(me.x), total); }
+      });
       return;
     }
     __syncthreads();
