@@ -88,6 +88,20 @@ __device__ __forceinline__ unsigned wave_scan_u32(unsigned v) {
   return v;
 }
 
+__device__ __forceinline__ u64 wave_scan_u64(u64 v) {
+#define DSRG_STEP(ctrl, rows)                                                                                  \
+  v += (u64)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), ctrl, rows, 0xF, true) << 32 |  \
+       (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, ctrl, rows, 0xF, true)
+  DSRG_STEP(0x111, 0xF);
+  DSRG_STEP(0x112, 0xF);
+  DSRG_STEP(0x114, 0xF);
+  DSRG_STEP(0x118, 0xF);
+  DSRG_STEP(0x142, 0xA);
+  DSRG_STEP(0x143, 0xC);
+#undef DSRG_STEP
+  return v;
+}
+
 template <typename T> __device__ __forceinline__ float load_logit(const T* row, int j) {
   const float x = Elem<T>::ld(row + j) + 0.0f;          // (-0 + 0 = +0: the two zeros are one value)
   return x != x ? -INFINITY : x;
@@ -107,6 +121,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   __shared__ double tab[32];
   __shared__ u64 red_a[NW], red_b[NW];
   __shared__ float s_max[NW], s_valid[NW];
+  __shared__ double s_c2, s_tlogm;
   __shared__ u64 s_thr, s_base_m, s_base_c, s_bin_m;
   __shared__ unsigned s_bin, s_n, s_bin_n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
@@ -114,7 +129,6 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
   const int Kk = a.topk ? a.topk[b] : a.topk0;
   const float u_raw = a.u[b], uu = u_raw >= 0.f ? fminf(u_raw, 0.99999994f) : 0.f;
-  if (tid < 32) tab[tid] = EXP2_32[tid];
   // wave w's part of the row: index order is (wave, step, lane)
   const int seg = (V + NW * 64 - 1) / (NW * 64) * 64, j0 = min(V, w * seg), j1 = min(V, j0 + seg);
 
@@ -134,6 +148,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int i = 0; i < VPT; ++i) xs[i] = load_logit(row, min(j0 + i * 64 + lane, V - 1));
 #pragma unroll
     for (int i = 0; i < VPT; ++i) xs[i] = j0 + i * 64 + lane < j1 ? xs[i] : -INFINITY;
+  }
+  // (while the row is on its way)
+  if (tid < 32) tab[tid] = EXP2_32[tid];
+  if (tid == NT - 1) {
+    s_c2 = 32 * 1.44269504088896340736 / (double)Tm;
+    s_tlogm = M > 0.f ? (double)Tm * log((double)M) : -INFINITY;
   }
   auto each = [&](auto&& f) {
     if constexpr (VPT > 0) {
@@ -168,7 +188,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     if (tid == 0) { a.token[b] = (int)s_n; a.logp[b] = 0.f; }
     return;
   }
-  const double c2 = 32 * 1.44269504088896340736 / (double)Tm;
+  const double c2 = s_c2, floor_ = (double)mx + s_tlogm;          // w >= m  <=>  x >= max + T ln m
   auto weight = [&](float x) -> u64 { return x == mx ? (u64)1 << WBITS : fixed_exp2(((double)x - (double)mx) * c2, tab); };
   auto logp_of = [&](float x, u64 total) -> float {
     return (float)((x == mx ? 0.0 : ((double)x - (double)mx) / (double)Tm) - log(ldexp((double)total, -WBITS)));
@@ -181,7 +201,6 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     const unsigned lo = 0x3b800000u >> SH;              // 2^-8
     return d < lo ? 0u : min(d - lo, (unsigned)NB - 1);
   };
-  const double floor_ = M > 0.f ? (double)mx + (double)Tm * log((double)M) : -INFINITY;        // w >= m  <=>  x >= max + T ln m
 
   // For every entry of the list, by the 16 lanes of a DPP row together: how many entries `ahead(other, me)` holds for and what they weigh.
   auto ranked = [&](int n, auto&& ahead, auto&& f) {
@@ -211,12 +230,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     u64 tc = 0, tm = 0;
 #pragma unroll
     for (int i = 0; i < BPT; ++i) { tc += cnt[tid * BPT + i]; tm += mass[tid * BPT + i]; }
-    u64 ic = tc, im = tm;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 yc = __shfl_up(ic, o), ym = __shfl_up(im, o);
-      if (lane >= o) { ic += yc; im += ym; }
-    }
+    u64 ic = wave_scan_u32((unsigned)tc), im = by_mass ? wave_scan_u64(tm) : 0;
     if (lane == 63) { red_a[w] = ic; red_b[w] = im; }
     __syncthreads();
     u64 bc = c0, bm = m0, total = 0;
@@ -329,13 +343,54 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     __syncthreads();
   };
 
+  // The rest, once the list holds everything that can still be drawn (s_n entries, weights not yet filled in): the first `want`, of them
+  // what top-p keeps (p >= 1: all), of them what min-p keeps, and the draw.
+  auto draw_from_list = [&](unsigned want, float p) {
+    const int n = (int)s_n;
+    auto value = [&](u64 comp) { return of_key((unsigned)(comp >> 32)); };
+    for (int i = tid; i < n; i += NT) list[i].y = weight(value(list[i].x));
+    __syncthreads();
+    // rank and the weight ahead of every entry; what the first `want` weigh (only top-p asks for it)
+    u64 sum = 0;
+    ranked(n, larger, [&](int i, const ulonglong2& me, unsigned c, u64 m) {
+      l_rank[i] = c;
+      l_ahead[i] = m;
+      if (c < want) sum += me.y;
+    });
+    sum = wave_sum_u64(sum);
+    if (lane == 0) red_a[w] = sum;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) all += red_a[i];
+    const double goal = fmax((double)p, 0.0) * (double)all;
+    sum = 0;
+    for (int i = tid; i < n; i += NT) {                 // what is not kept loses its weight: it is not drawn then
+      const ulonglong2 me = list[i];
+      const float x = value(me.x);
+      const unsigned rank = l_rank[i];
+      const bool keep = rank == 0 || (rank < want && (!(p < 1.f) || (double)l_ahead[i] < goal) && (x == mx || (double)x >= floor_));
+      if (keep) sum += me.y; else list[i].y = 0;
+    }
+    sum = wave_sum_u64(sum);
+    if (lane == 0) red_b[w] = sum;
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) total += red_b[i];
+    const double draw = (double)uu * (double)total;
+    // (the low word is ~index: the entries before have a larger one)
+    ranked(n, [](const ulonglong2& o, const ulonglong2& me) { return (unsigned)o.x > (unsigned)me.x; }, [&](int, const ulonglong2& me, unsigned, u64 m) {
+      if (me.y && (double)m <= draw && (double)(m + me.y) > draw) { a.token[b] = (int)~(unsigned)me.x; a.logp[b] = logp_of(value(me.x), total); }
+    });
+  };
+
   // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
   // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
   // wanted ones, and few others.  One bin a thread here (NT / 16 an octave): a bin costs a few more entries, a scan more costs time.
   const bool small = VPT == 1, few = Kk > 0 && Kk <= 256 && Kk < nvalid;
   if (small || few) {
-    float edge = 0.f;                                   // the candidates with max - x < edge, or every one
-    bool every = true;
+    float lim = -3.4028235e38f;                         // entries from here on (every candidate: -inf and NaN are none)
     if (tid == 0) s_n = 0;
     if (!small) {
       constexpr int SN = 23 - (NT == 1024 ? 6 : 4);
@@ -358,66 +413,62 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       if (ic >= (unsigned)Kk && ic - tc < (unsigned)Kk) s_bin = tid;
       __syncthreads();
       const unsigned last = s_bin;
-      every = last >= NT - 1;
-      if (!every) edge = __uint_as_float((last + lo + 1) << SN);
+      // fl(max - x) < edge means max - x < edge (1 + 2^-24): all of those are above this, rounded down by 2^-22 of edge and of the result
+      if (last < NT - 1) {
+        const double edge = __uint_as_float((last + lo + 1) << SN), at = (double)mx - edge * (1.0 + 0x1p-22);
+        lim = fmaxf((float)(at - fabs(at) * 0x1p-22), lim);
+      }
     } else __syncthreads();
-    each([&](float x, int j) {
-      if (every ? x > -INFINITY : x == mx || mx - x < edge) {
+    auto take = [&](float x, int j) {
+      if (x >= lim) {
+        const unsigned at = atomicAdd(&s_n, 1u);
+        if (at < LIST) list[at].x = comp_of(x, j);
+      }
+    };
+    if constexpr (VPT >= 8) {
+#pragma unroll
+      for (int i = 0; i < VPT; i += 8) {                // (one test for eight: few of a wave's 512 are taken)
+        float m = xs[i];
+#pragma unroll
+        for (int t = 1; t < 8; ++t) m = fmaxf(m, xs[i + t]);
+        if (__any(m >= lim))
+#pragma unroll
+          for (int t = 0; t < 8; ++t) take(xs[i + t], j0 + (i + t) * 64 + lane);
+      }
+    } else each(take);
+    __syncthreads();
+    if (s_n <= LIST) {
+      draw_from_list(Kk > 0 ? (unsigned)Kk : ~0u, P);
+      return;
+    }
+    __syncthreads();
+  }
+  u64 certain = 0;                                      // entries that are left at least
+  if (Kk > 0 && Kk < nvalid) { cut(false, (u64)Kk, 0.0); certain = Kk; }
+  if (P < 1.f) { cut(true, 0, (double)P); certain = s_base_c; }
+  auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
+  __syncthreads();
+
+  // what is left, where that is little
+  constexpr int SHORT = NT / 4;                         // (ranks cost n^2 / NT, another pass of weights V / NT)
+  if ((thr || M > 0.f) && certain <= SHORT) {
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    again([&](float x, int j) {
+      if (kept(x, j)) {
         const unsigned at = atomicAdd(&s_n, 1u);
         if (at < LIST) list[at].x = comp_of(x, j);
       }
     });
     __syncthreads();
-    const int n = (int)s_n;
-    if (n <= LIST) {
-      auto value = [&](u64 comp) { return of_key((unsigned)(comp >> 32)); };
-      for (int i = tid; i < n; i += NT) list[i].y = weight(value(list[i].x));
-      __syncthreads();
-      const unsigned want = Kk > 0 ? (unsigned)Kk : ~0u;
-      // rank and the weight ahead of every entry; what the first want ones weigh (only top-p asks for it)
-      u64 sum = 0;
-      ranked(n, larger, [&](int i, const ulonglong2& me, unsigned c, u64 m) {
-        l_rank[i] = c;
-        l_ahead[i] = m;
-        if (c < want) sum += me.y;
-      });
-      sum = wave_sum_u64(sum);
-      if (lane == 0) red_a[w] = sum;
-      __syncthreads();
-      u64 all = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) all += red_a[i];
-      const double goal = fmax((double)P, 0.0) * (double)all;
-      sum = 0;
-      for (int i = tid; i < n; i += NT) {               // what is not kept loses its weight: it is not drawn then
-        const ulonglong2 me = list[i];
-        const float x = value(me.x);
-        const unsigned rank = l_rank[i];
-        const bool keep = rank == 0 || (rank < want && (!(P < 1.f) || (double)l_ahead[i] < goal) && (x == mx || (double)x >= floor_));
-        if (keep) sum += me.y; else list[i].y = 0;
-      }
-      sum = wave_sum_u64(sum);
-      if (lane == 0) red_b[w] = sum;
-      __syncthreads();
-      u64 total = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) total += red_b[i];
-      const double draw = (double)uu * (double)total;
-      // (the low word is ~index: the entries before have a larger one)
-      ranked(n, [](const ulonglong2& o, const ulonglong2& me) { return (unsigned)o.x > (unsigned)me.x; }, [&](int, const ulonglong2& me, unsigned, u64 m) {
-        if (me.y && (double)m <= draw && (double)(m + me.y) > draw) { a.token[b] = (int)~(unsigned)me.x; a.logp[b] = logp_of(value(me.x), total); }
-      });
+    if (s_n <= SHORT) {
+      draw_from_list(~0u, 1.f);
       return;
     }
-    __syncthreads();
   }
-  if (Kk > 0 && Kk < nvalid) cut(false, (u64)Kk, 0.0);
-  if (P < 1.f) cut(true, 0, (double)P);
 
   // what is left, in index order
   u64 sum = 0;
-  auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
-  __syncthreads();
   again([&](float x, int j) {
     if (kept(x, j)) sum += weight(x);
   });
@@ -436,8 +487,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       if (!__ballot(in)) continue;
       u64 c = in ? weight(x) : 0;
       const u64 own = c;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(c, o); if (lane >= o) c += y; }
+      c = wave_scan_u64(c);
       const u64 hit = __ballot(own && (double)(base + c) > goal);
       if (hit) {
         if (lane == __builtin_ctzll(hit)) {
@@ -446,7 +496,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
         }
         break;
       }
-      base += __shfl(c, 63);
+      base += lane_u64(c, 63);
     }
   }
 }
