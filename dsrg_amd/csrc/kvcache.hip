@@ -318,8 +318,10 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
 
 // MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
 // UB: 32-token blocks a step, so that a step's keys and values are 8 KB or so each of a wave's loads whatever the type.
-// Workgroups of four waves that a CU holds: bounded by the registers of O, of the step's keys and values and of the queries.
+// Waves that a SIMD holds: bounded by the registers of O, of the step's keys and values and of the queries.
 constexpr int resident(int kv, int D, int CT) { return D == 64 ? (CT == 1 ? 4 : 3) - (kv == DSRG_F32) : kv == DSRG_F32 ? 1 : 2; }
+// Waves of a large workgroup (one column tile): all that a CU holds, so that a sequence's tokens are joined in LDS as far as that goes
+constexpr int most_waves(int kv, int D, int CT) { return CT > 1 ? 4 : kv == DSRG_F32 ? (D == 64 ? 12 : 4) : D == 64 ? 16 : 8; }
 // 32-token blocks a step (one 16-column tile; with two the registers do not hold more than one)
 constexpr int step_blocks(int kv, int D) { return D == 128 && (kv == DSRG_I8 || kv == DSRG_E4M3) ? 2 : 1; }
 template <int KV, int D, int CT, int NW, bool MIX, int UB>
@@ -330,8 +332,11 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
   constexpr int KS = F ? D / 16 : D / 32;        // 16-byte (8-byte) key chunks of a lane per 16-token tile
   constexpr int DT = D / 16;
   constexpr int OLD = D + 4;
-  __shared__ float so[NW][16][OLD];
-  __shared__ float sm[NW][16], sl[NW][16];
+  extern __shared__ __attribute__((aligned(16))) float smem[];               // [NW][nc][OLD], then the waves' maxima and sums [NW][nc] each
+  const int nc = min(16, a.NC);
+  float* const so = smem;
+  float* const sm = so + NW * nc * OLD;
+  float* const sl = sm + NW * nc;
   const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int sp = blockIdx.x, H = a.c.H, kh = blockIdx.y % H, cg = blockIdx.y / H, b = blockIdx.z;
   const int cap = a.width * a.c.S;
@@ -602,18 +607,27 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32((&vr[u][t * DT + dt].x)[i], s_[ct][u][t][i], o[ct][dt], 0, 0, 0);
       } else {
-        bf16x8 pf[CT];
+        // P as the sum of two bf16 numbers (16 bits of it): the matrix units wait for memory, and one rounding of P to 8 bits would be as
+        // large an error as the output's own
+        bf16x8 pf[CT], pl[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pf[ct][j] = (__bf16)s_[ct][u][j >> 2][j & 3];
+          for (int j = 0; j < 8; ++j) {
+            const float x = s_[ct][u][j >> 2][j & 3];
+            pf[ct][j] = (__bf16)x;
+            pl[ct][j] = (__bf16)(x - (float)pf[ct][j]);
+          }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           bf16x8 vf;
           if constexpr (Q8) vf = codes_to_bf16(vr[u][dt], KV);
           else vf = __builtin_bit_cast(bf16x8, vr[u][dt]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct], o[ct][dt], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) {
+            o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[ct], o[ct][dt], 0, 0, 0);
+            o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[ct], o[ct][dt], 0, 0, 0);
+          }
         }
       }
     }
@@ -627,24 +641,24 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
     if (ct) __syncthreads();
     const float ls = col_sum(l[ct]);
     if (c16 < nv) {
-      if (g == 0) { sm[w][c16] = m[ct]; sl[w][c16] = ls; }
+      if (g == 0) { sm[w * nc + c16] = m[ct]; sl[w * nc + c16] = ls; }
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(&so[w][c16][dt * 16 + 4 * g]) = o[ct][dt];
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(so + (w * nc + c16) * OLD + dt * 16 + 4 * g) = o[ct][dt];
     }
     __syncthreads();
     for (int idx = threadIdx.x; idx < nv * (D / 4); idx += NW * 64) {
       const int c = idx / (D / 4), d = (idx % (D / 4)) * 4, n = n0 + c;
       float M = -INFINITY;
 #pragma unroll
-      for (int ww = 0; ww < NW; ++ww) M = fmaxf(M, sm[ww][c]);
+      for (int ww = 0; ww < NW; ++ww) M = fmaxf(M, sm[ww * nc + c]);
       float L = 0.f;
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ww = 0; ww < NW; ++ww) {
-        const float f = sm[ww][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[ww][c] - M);
+        const float mw = sm[ww * nc + c], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
         if (f != 0.f) {
-          L += f * sl[ww][c];
-          O += f * *reinterpret_cast<const f32x4*>(&so[ww][c][d]);
+          L += f * sl[ww * nc + c];
+          O += f * *reinterpret_cast<const f32x4*>(so + (ww * nc + c) * OLD + d);
         }
       }
       if (a.nsplit == 1) {
@@ -728,17 +742,19 @@ int check_table(const char* who, const int32_t* table, int ld, int width, int S,
 }
 bool rows16(const void* p, long long bs, long long rs, int size) { return (uintptr_t)p % 16 == 0 && bs * size % 16 == 0 && rs * size % 16 == 0; }
 
-struct Split { int nsplit, bps; };
-// The tokens of a sequence are split so that the workgroups fill the chip's places (256 CUs) about once: fewer leave CUs idle, more than fit
-// wait for a second round and have to be joined all the same.  A workgroup gets 256 tokens at least (below, the join costs more than it
-// saves), and 16384 at most, so that one long sequence among short ones does not run alone for long.
+struct Split { int nw, nsplit, bps; };
+// How many waves share a sequence's tokens (per key / value head and column group): as many as fill the chip's places (1024 SIMDs) about
+// once (more than fit would wait for a second round), each with 64 tokens at least; at most 16384 tokens a workgroup, so that one long sequence among short ones does not run alone for
+// long.  Waves of a workgroup are joined in LDS, workgroups by a second kernel (4 to 5 us more): large workgroups where four waves are
+// not enough, and splits only where one of them is not.
 Split plan_split(int kv, int D, int ct, int B, int H, int cgs, long long max_tokens) {
-  const long long blocks = (max_tokens + 31) / 32, have = (long long)B * H * cgs, places = 256ll * resident(kv, D, ct);
-  long long ns = (2 * places + have) / (2 * have);
-  ns = std::min(std::max(ns, (blocks + 511) / 512), (blocks + 7) / 8);
+  const long long blocks = std::max((max_tokens + 31) / 32, 1ll), have = (long long)B * H * cgs, places = 1024ll * resident(kv, D, ct), most = most_waves(kv, D, ct);
+  const long long waves = std::max(std::min(places / have, (blocks + 1) / 2), 4ll);
+  const long long nw = waves >= 6 ? most : 4;
+  long long ns = std::max(waves / nw, (blocks + 511) / 512);
   ns = std::min(std::max(ns, 1ll), 1024ll);
-  const long long bps = std::max((blocks + ns - 1) / ns, 1ll);
-  return Split{(int)std::max((blocks + bps - 1) / bps, 1ll), (int)bps};
+  const long long bps = (blocks + ns - 1) / ns;
+  return Split{(int)nw, (int)((blocks + bps - 1) / bps), (int)bps};
 }
 long long seen_tokens(int width, int S, int Nq, int window) {
   const long long cap = (long long)width * S;
@@ -749,6 +765,11 @@ long long seen_tokens(int width, int S, int Nq, int window) {
 int col_tiles(int NC) { return NC > 16 ? 2 : 1; }
 
 }  // namespace
+
+template <int KV, int D, int CT, int NW, bool MIX, int UB> static void launch_paged(const PagedArgs& a, dim3 grid, int lds, hipStream_t st) {
+  if (NW * 16 * (D + 6) * 4 > 65536) DSRG_SET_MAX_LDS_ONCE((attention_paged_kernel<KV, D, CT, NW, MIX, UB>), NW * 16 * (D + 6) * 4);
+  hipLaunchKernelGGL((attention_paged_kernel<KV, D, CT, NW, MIX, UB>), grid, dim3(NW * 64), lds, st, a);
+}
 
 #define KV_SWITCH(DT, ...)                                               \
   switch (DT) {                                                          \
@@ -866,22 +887,30 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   a.causal = causal != 0; a.window = window; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
   a.ws_o = (float*)workspace;
   a.ws_ml = need ? (float2*)((float*)workspace + (int64_t)B * a.c.H * a.NC * s.nsplit * D_) : nullptr;
-  const dim3 grid(s.nsplit, a.c.H * cgs, B), block(256);
+  const dim3 grid(s.nsplit, a.c.H * cgs, B);
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
-        if (mix && ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, true, step_blocks(KV, D)>), grid, block, 0, st, a);
-    else if (mix) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, true, 1>), grid, block, 0, st, a);
-    else if (ct == 1) hipLaunchKernelGGL((attention_paged_kernel<KV, D, 1, 4, false, step_blocks(KV, D)>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attention_paged_kernel<KV, D, 2, 4, false, 1>), grid, block, 0, st, a);
+        constexpr int MW = most_waves(KV, D, 1), UB = step_blocks(KV, D);
+    const int lds = s.nw * std::min(16, a.NC) * (D + 6) * 4;
+    if (ct == 2) {
+      if (mix) launch_paged<KV, D, 2, 4, true, 1>(a, grid, lds, st);
+      else launch_paged<KV, D, 2, 4, false, 1>(a, grid, lds, st);
+    } else if (s.nw == 4) {
+      if (mix) launch_paged<KV, D, 1, 4, true, UB>(a, grid, lds, st);
+      else launch_paged<KV, D, 1, 4, false, UB>(a, grid, lds, st);
+    } else {
+      if (mix) launch_paged<KV, D, 1, MW, true, UB>(a, grid, lds, st);
+      else launch_paged<KV, D, 1, MW, false, UB>(a, grid, lds, st);
+    }
   }))
   DSRG_LAUNCH_CHECK("dsrg_attention_paged");
   if (s.nsplit > 1) {
     const long long rows = (long long)B * a.c.H * a.NC;
     const dim3 jgrid((unsigned)((rows + 3) / 4));
     D_SWITCH(D_, {
-      if (dtype == DSRG_F32) hipLaunchKernelGGL((attention_paged_join_kernel<D, float>), jgrid, block, 0, st, a);
-      else hipLaunchKernelGGL((attention_paged_join_kernel<D, bf16_t>), jgrid, block, 0, st, a);
+      if (dtype == DSRG_F32) hipLaunchKernelGGL((attention_paged_join_kernel<D, float>), jgrid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((attention_paged_join_kernel<D, bf16_t>), jgrid, dim3(256), 0, st, a);
     })
     DSRG_LAUNCH_CHECK("dsrg_attention_paged (join)");
   }

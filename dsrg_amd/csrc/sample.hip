@@ -34,26 +34,38 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ u64 comp_of(float x, int j) { return ((u64)key_of(x) << 32) | (unsigned)~j; }
 
-__constant__ const double EXP2_32[32] = {      // 2^(k / 32)
+__constant__ const double EXP2_A[32] = {       // 2^(k / 32)
     1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
     1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
     1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
     1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543,
     1.6457554781539649, 1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424,
     1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__constant__ const double EXP2_B[32] = {       // 2^(k / 1024)
+    1, 1.0006771306930664, 1.0013547198921082, 1.002032767907594, 1.0027112750502025, 1.0033902416308227,
+    1.0040696679605541, 1.0047495543507072, 1.0054299011128027, 1.006110708558573, 1.0067919769999607, 1.0074737067491204,
+    1.0081558981184175, 1.0088385514204294, 1.0095216669679448, 1.0102052450739643, 1.0108892860517005,
+    1.0115737902145781, 1.0122587578762337, 1.0129441893505169, 1.0136300849514894, 1.0143164449934257,
+    1.0150032697908125, 1.0156905596583505, 1.0163783149109531, 1.0170665358637463, 1.0177552228320703,
+    1.0184443761314785, 1.0191339960777379, 1.0198240829868295, 1.0205146371749483, 1.0212056589585028};
+// 2^(k / 1024) as a fixed-point number with 62 bits behind the point
+__device__ __forceinline__ u64 exp2_table(int k) {
+  const u64 bits = (u64)__double_as_longlong(EXP2_A[k >> 5] * EXP2_B[k & 31]);
+  return ((bits & 0xfffffffffffffull) | 0x10000000000000ull) << 10;
+}
 
-// 2^(t32 / 32) in WBITS-bit fixed point for t32 <= 0: 2^(n/32) from a table, the rest as e^y, |y| <= ln2 / 64, by its series (the
-// first term left out is y^5 / 120 < 1.3e-12 of the weight).  Adding 2^(52 - WBITS) leaves the rounded fixed-point number in the mantissa.
-__device__ __forceinline__ u64 fixed_exp2(double t32, const double* tab) {
-  if (!(t32 > -46.0 * 32)) return 0;
-  const double s = rint(t32), y = (t32 - s) * (0.69314718055994530942 / 32);
-  const int n = (int)s;
-  double e = fma(y, 1.0 / 24.0, 1.0 / 6.0);
-  e = fma(y, e, 0.5);
-  e = fma(y, e, 1.0);
-  e = fma(y, e, 1.0);
-  constexpr double MAGIC = (double)(1ull << (52 - WBITS));
-  return (u64)__double_as_longlong(ldexp(e * tab[n & 31], n >> 5) + MAGIC) - (u64)__builtin_bit_cast(long long, MAGIC);
+// 2^(t / 1024) in WBITS-bit fixed point for t <= 0.  With k the whole number next to t, 2^(k / 1024) comes from the table and a shift, and
+// e^y, |y| <= ln2 / 2048, is 1 + (y + y^2 / 2): the first term left out is y^3 / 6 < 7e-12, and the bracket, 2^-11 of the result at most, is
+// fine in fp32 (2^-35 of it).  Adding 1.5 * 2^52 leaves k in the low word.
+__device__ __forceinline__ u64 fixed_exp2(double t, const u64* tab) {
+  constexpr double MAGIC = 0x1.8p52;
+  t = fmax(t, -65536.0);
+  const double kk = t + MAGIC;
+  const int k = (int)(unsigned)(u64)__double_as_longlong(kk);
+  const float y = (float)(t - (kk - MAGIC)) * (float)(0.69314718055994530942 / 1024);
+  const u64 T = tab[k & 1023];
+  const float more = fmaf(y * 0.5f, y, y) * ((float)(unsigned)(T >> 32) * 256.f);        // in units of 2^24
+  return (u64)((long long)T + ((long long)(int)more << 24)) >> min(62 - WBITS - (k >> 10), 63);
 }
 
 template <int CTRL> __device__ __forceinline__ u64 dpp_u64(u64 v) {
@@ -118,12 +130,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   u64* const l_ahead = mass;                            // (the short way has no use for the bins' weights)
   unsigned* const l_rank = cnt;
   static_assert(NB >= LIST, "one word an entry");
-  __shared__ double tab[32];
+  __shared__ u64 tab[1024];
   __shared__ u64 red_a[NW], red_b[NW];
   __shared__ float s_max[NW], s_valid[NW];
   __shared__ double s_c2, s_tlogm;
-  __shared__ u64 s_thr, s_base_m, s_base_c, s_bin_m;
-  __shared__ unsigned s_bin, s_n, s_bin_n;
+  __shared__ u64 s_thr, s_base, s_bin_v;
+  __shared__ unsigned s_bin, s_n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
   const T* row = (const T*)a.logits + (long long)b * a.ld;
   const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
@@ -150,9 +162,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int i = 0; i < VPT; ++i) xs[i] = j0 + i * 64 + lane < j1 ? xs[i] : -INFINITY;
   }
   // (while the row is on its way)
-  if (tid < 32) tab[tid] = EXP2_32[tid];
+  for (int k = tid; k < 1024; k += NT) tab[k] = exp2_table(k);
   if (tid == NT - 1) {
-    s_c2 = 32 * 1.44269504088896340736 / (double)Tm;
+    s_c2 = 1024 * 1.44269504088896340736 / (double)Tm;
     s_tlogm = M > 0.f ? (double)Tm * log((double)M) : -INFINITY;
   }
   auto each = [&](auto&& f) {
@@ -202,52 +214,69 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     return d < lo ? 0u : min(d - lo, (unsigned)NB - 1);
   };
 
-  // For every entry of the list, by the 16 lanes of a DPP row together: how many entries `ahead(other, me)` holds for and what they weigh.
+  // For every entry of the list: what the entries weigh for which `ahead(other, me)` holds, and how many they are.  The 16 lanes of a DPP row
+  // share four entries and walk the list together.
   auto ranked = [&](int n, auto&& ahead, auto&& f) {
+    constexpr int EB = 4;
     const int sub = tid & 15;
-    for (int i0 = 0; i0 < n; i0 += NT / 16) {
-      const int i = i0 + (tid >> 4);
-      const ulonglong2 me = list[min(i, n - 1)];
-      unsigned c = 0;
-      u64 m = 0;
-#pragma unroll 4
+    for (int i0 = 0; i0 < n; i0 += NT / 16 * EB) {
+      const int i1 = i0 + (tid >> 4) * EB;
+      if (__builtin_amdgcn_readfirstlane(i1) >= n) break;                // (the wave's lowest entry)
+      ulonglong2 me[EB];
+      unsigned c[EB];
+      u64 m[EB];
+#pragma unroll
+      for (int e = 0; e < EB; ++e) { me[e] = list[min(i1 + e, n - 1)]; c[e] = 0; m[e] = 0; }
+#pragma unroll 2
       for (int k = sub; k < n; k += 16) {
         const ulonglong2 o = list[k];
-        const bool up = ahead(o, me);
-        c += up;
-        m += up ? o.y : 0;
+#pragma unroll
+        for (int e = 0; e < EB; ++e) {
+          const bool up = ahead(o, me[e]);
+          c[e] += up;
+          m[e] += up ? o.y : 0;
+        }
       }
-      const u64 cs = row_sum_u64(c);
-      m = row_sum_u64(m);
-      if (sub == 0 && i < n) f(i, me, (unsigned)cs, m);
+#pragma unroll
+      for (int e = 0; e < EB; ++e) {
+        const unsigned cs = (unsigned)row_sum_u64(c[e]);
+        const u64 ms = row_sum_u64(m[e]);
+        if (sub == e && i1 + e < n) f(i1 + e, me[e], cs, ms);
+      }
     }
   };
   auto larger = [](const ulonglong2& o, const ulonglong2& me) { return o.x > me.x; };
-  // Running count and weight over the bins, behind (c0, m0); the first bin that reaches the goal goes to s_bin, with what lies
-  // before it and what it holds.  *goal < 0: it is frac of what all bins weigh.  (Entries so far down that their weight rounds to
-  // 0 never reach a goal: the last bin that weighs anything does.)
-  auto locate = [&](bool by_mass, u64 want, double frac, u64 c0, u64 m0, double* goal) {
-    u64 tc = 0, tm = 0;
+  auto clear = [&](bool by_mass) {
+    for (int i = tid; i < NB; i += NT)
+      if (by_mass) mass[i] = 0; else cnt[i] = 0;
+  };
+  auto put = [&](bool by_mass, unsigned bin, float x) {
+    if (by_mass) atomicAdd(&mass[bin], weight(x)); else atomicAdd(&cnt[bin], 1u);
+  };
+  // Running sum over the bins (of counts or of weights), behind what lies before them; the first bin at which it reaches the goal goes to
+  // s_bin, with what lies before it.  *goal < 0: it is frac of the whole.  By weight the first entry is inside whatever the goal (it weighs
+  // most; nothing weighs anything before it), and a bin whose weights all rounded to 0 never reaches one.
+  auto locate = [&](bool by_mass, u64 want, double frac, u64 before, double* goal) {
+    u64 t = 0;
 #pragma unroll
-    for (int i = 0; i < BPT; ++i) { tc += cnt[tid * BPT + i]; tm += mass[tid * BPT + i]; }
-    u64 ic = wave_scan_u32((unsigned)tc), im = by_mass ? wave_scan_u64(tm) : 0;
-    if (lane == 63) { red_a[w] = ic; red_b[w] = im; }
+    for (int i = 0; i < BPT; ++i) t += by_mass ? mass[tid * BPT + i] : cnt[tid * BPT + i];
+    u64 inc = by_mass ? wave_scan_u64(t) : wave_scan_u32((unsigned)t);
+    if (lane == 63) red_a[w] = inc;
     __syncthreads();
-    u64 bc = c0, bm = m0, total = 0;
-    for (int i = 0; i < NW; ++i) { if (i < w) { bc += red_a[i]; bm += red_b[i]; } total += red_b[i]; }
-    ic += bc; im += bm;
-    u64 ec = ic - tc, em = im - tm;
+    u64 total = 0;
+    inc += before;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) { inc += i < w ? red_a[i] : 0; total += red_a[i]; }
+    u64 ex = inc - t;
     if (*goal < 0) *goal = fmax(frac, 0.0) * (double)total;
-    if (tc && (by_mass ? ((double)em < *goal || ec == 0) && (double)im >= *goal : ec < want && ic >= want)) {
+    auto reached = [&](u64 v) { return by_mass ? (double)v >= *goal && v : v >= want; };
+    if (t && !reached(ex) && reached(inc)) {
       bool done = false;
 #pragma unroll
       for (int i = 0; i < BPT; ++i) {
-        const u64 nc = cnt[tid * BPT + i], nm = mass[tid * BPT + i];
-        if (!done && nc && (by_mass ? (double)(em + nm) >= *goal : ec + nc >= want)) {
-          done = true;
-          s_bin = tid * BPT + i; s_base_c = ec; s_base_m = em; s_bin_n = (unsigned)nc; s_bin_m = nm;
-        }
-        ec += nc; em += nm;
+        const u64 v = by_mass ? mass[tid * BPT + i] : cnt[tid * BPT + i];
+        if (!done && reached(ex + v)) { done = true; s_bin = tid * BPT + i; s_base = ex; s_bin_v = v; }
+        ex += v;
       }
     }
     __syncthreads();
@@ -256,31 +285,38 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   // One cut: by_mass false: after `want` entries; true: after the first whose running weight reaches frac of the whole.
   auto cut = [&](bool by_mass, u64 want, double frac) {
     double goal = -1.0;
-    for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
+    clear(by_mass);
     if (tid == 0) { s_thr = ~0ull; s_n = 0; }
     __syncthreads();
     again([&](float x, int j) {
-      if (x > -INFINITY && comp_of(x, j) >= thr) {
-        const unsigned bin = bin_of(x);
-        atomicAdd(&cnt[bin], 1u);
-        if (by_mass) atomicAdd(&mass[bin], weight(x));
-      }
+      if (x > -INFINITY && comp_of(x, j) >= thr) put(by_mass, bin_of(x), x);
     });
     __syncthreads();
-    locate(by_mass, want, frac, 0, 0, &goal);
+    locate(by_mass, want, frac, 0, &goal);
     const unsigned bin = s_bin;
-    u64 base_c = s_base_c, base_m = s_base_m;
-    if (s_bin_n <= LIST) {
-      again([&](float x, int j) {
-        if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin) {
+    u64 base = s_base;
+    // the bin's entries: values between its edges, widened a little for the rounding of max - x, then looked at exactly
+    constexpr unsigned BLO = 0x3b800000u >> SH;
+    const double e0 = bin ? (double)__uint_as_float((bin + BLO) << SH) : 0.0, e1 = bin < NB - 1 ? (double)__uint_as_float((bin + BLO + 1) << SH) : INFINITY;
+    const double slack = fabs((double)mx) * 0x1p-22, top = (double)mx - e0 * (1.0 - 0x1p-22) + slack, bottom = (double)mx - e1 * (1.0 + 0x1p-22) - slack;
+    const float vtop = top < 3.4e38 ? (float)top : INFINITY, vbottom = bottom > -3.4e38 ? (float)bottom : -3.4028235e38f;
+    const bool exact_only = !(fabs((double)mx) < 3e38);
+    {
+      each([&](float x, int j) {
+        if ((exact_only ? x > -INFINITY : x >= vbottom && x <= vtop) && bin_of(x) == bin && comp_of(x, j) >= thr) {
           const unsigned at = atomicAdd(&s_n, 1u);
-          list[at] = make_ulonglong2(comp_of(x, j), by_mass ? weight(x) : 0);
+          if (at < LIST) list[at].x = comp_of(x, j);
         }
       });
       __syncthreads();
-      const int n = (int)s_n;
-      ranked(n, larger, [&](int, const ulonglong2& me, unsigned c, u64 m) {
-        if (by_mass ? (double)(base_m + m) < goal || base_c + c == 0 : base_c + c < want) atomicMin(&s_thr, me.x);
+    }
+    const int n = (int)s_n;
+    if (n <= LIST) {
+      for (int i = tid; i < n; i += NT) list[i].y = by_mass ? weight(of_key((unsigned)(list[i].x >> 32))) : 1;
+      __syncthreads();
+      ranked(n, larger, [&](int, const ulonglong2& me, unsigned, u64 m) {
+        const u64 ahead = base + m;
+        if (by_mass ? (double)ahead < goal || ahead == 0 : ahead < want) atomicMin(&s_thr, me.x);
       });
       __syncthreads();
       thr = s_thr;
@@ -291,34 +327,29 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       for (int sh = 32; sh > 0;) {
         const int nb = min(LB, sh);
         sh -= nb;
-        for (int i = tid; i < NB; i += NT) { cnt[i] = 0; mass[i] = 0; }
+        clear(by_mass);
         __syncthreads();
         again([&](float x, int j) {
           const unsigned k = key_of(x);
-          if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin && (k & pmask) == prefix) {
-            const unsigned dig = ~(k >> sh) & ((1u << nb) - 1);            // falling values
-            atomicAdd(&cnt[dig], 1u);
-            if (by_mass) atomicAdd(&mass[dig], weight(x));
-          }
+          if (x > -INFINITY && comp_of(x, j) >= thr && bin_of(x) == bin && (k & pmask) == prefix) put(by_mass, ~(k >> sh) & ((1u << nb) - 1), x);       // falling values
         });
         __syncthreads();
-        locate(by_mass, want, frac, base_c, base_m, &goal);
-        base_c = s_base_c; base_m = s_base_m;
+        locate(by_mass, want, frac, base, &goal);
+        base = s_base;
         prefix |= (~s_bin & ((1u << nb) - 1)) << sh;
         pmask |= ((1u << nb) - 1) << sh;
         __syncthreads();
       }
-      // s_bin_n equal values of weight s_bin_m / s_bin_n: as many of them as the goal asks, the lowest indices first
+      // what is left are equal values: as many of them as the goal asks, the lowest indices first
+      const u64 one = by_mass ? weight(of_key(prefix)) : 1, ties = s_bin_v / one;
       u64 r;
-      const u64 each = s_bin_m / s_bin_n;
       if (by_mass) {
-        const double left = goal - (double)base_m;
-        r = each && left > 0 ? (u64)ceil(left / (double)each) : 1;
-        while (r > 1 && (double)(base_m + (r - 1) * each) >= goal) --r;
-        while ((double)(base_m + r * each) < goal && r < s_bin_n) ++r;
-      } else r = want - base_c;
-      if (r < 1) r = 1;
-      if (r > s_bin_n) r = s_bin_n;
+        const double left = goal - (double)base;
+        r = left > 0 ? (u64)ceil(left / (double)one) : 1;
+        while (r > 1 && (double)(base + (r - 1) * one) >= goal) --r;
+        while ((double)(base + r * one) < goal && r < ties) ++r;
+      } else r = want - base;
+      r = r < 1 ? 1 : r > ties ? ties : r;
       unsigned mine = 0;
       for (int j = j0 + lane; j - lane < j1; j += 64) mine += __popcll(__ballot(j < j1 && key_of(load_logit(row, j < V ? j : V - 1)) == prefix));
       if (lane == 0) red_a[w] = mine;
@@ -352,23 +383,27 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     __syncthreads();
     // rank and the weight ahead of every entry; what the first `want` weigh (only top-p asks for it)
     u64 sum = 0;
-    ranked(n, larger, [&](int i, const ulonglong2& me, unsigned c, u64 m) {
-      l_rank[i] = c;
-      l_ahead[i] = m;
-      if (c < want) sum += me.y;
-    });
-    sum = wave_sum_u64(sum);
-    if (lane == 0) red_a[w] = sum;
-    __syncthreads();
-    u64 all = 0;
+    const bool cuts = want < (unsigned)n || p < 1.f;
+    double goal = 0.0;
+    if (cuts) {
+      ranked(n, larger, [&](int i, const ulonglong2& me, unsigned c, u64 m) {
+        l_rank[i] = c;
+        l_ahead[i] = m;
+        if (c < want) sum += me.y;
+      });
+      sum = wave_sum_u64(sum);
+      if (lane == 0) red_a[w] = sum;
+      __syncthreads();
+      u64 all = 0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) all += red_a[i];
-    const double goal = fmax((double)p, 0.0) * (double)all;
-    sum = 0;
+      for (int i = 0; i < NW; ++i) all += red_a[i];
+      goal = fmax((double)p, 0.0) * (double)all;
+      sum = 0;
+    }
     for (int i = tid; i < n; i += NT) {                 // what is not kept loses its weight: it is not drawn then
       const ulonglong2 me = list[i];
       const float x = value(me.x);
-      const unsigned rank = l_rank[i];
+      const unsigned rank = cuts ? l_rank[i] : 1u;      // (the first one stays, as min-p keeps its equals)
       const bool keep = rank == 0 || (rank < want && (!(p < 1.f) || (double)l_ahead[i] < goal) && (x == mx || (double)x >= floor_));
       if (keep) sum += me.y; else list[i].y = 0;
     }
@@ -443,31 +478,35 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     }
     __syncthreads();
   }
-  u64 certain = 0;                                      // entries that are left at least
-  if (Kk > 0 && Kk < nvalid) { cut(false, (u64)Kk, 0.0); certain = Kk; }
-  if (P < 1.f) { cut(true, 0, (double)P); certain = s_base_c; }
+  if (Kk > 0 && Kk < nvalid) cut(false, (u64)Kk, 0.0);
+  if (P < 1.f) cut(true, 0, (double)P);
   auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
   __syncthreads();
 
-  // what is left, where that is little
-  constexpr int SHORT = NT / 4;                         // (ranks cost n^2 / NT, another pass of weights V / NT)
-  if ((thr || M > 0.f) && certain <= SHORT) {
+  // what is left, in index order: each wave's part is summed; little of it in all is drawn from a list
+  constexpr unsigned SHORT = NT / 4;                    // (ranks cost n^2 / NT)
+  if (thr || M > 0.f) {
     if (tid == 0) s_n = 0;
     __syncthreads();
-    again([&](float x, int j) {
-      if (kept(x, j)) {
-        const unsigned at = atomicAdd(&s_n, 1u);
-        if (at < LIST) list[at].x = comp_of(x, j);
-      }
-    });
+    // (a float below which nothing is kept: the smallest value the threshold lets through, or min-p's; the largest entry always is)
+    const float least = fminf(mx, fmaxf(thr ? of_key((unsigned)(thr >> 32)) : -3.4028235e38f, (float)(floor_ - fabs(floor_) * 0x1p-22)));
+    float over = 0.f;
+    each([&](float x, int) { over += x >= least ? 1.f : 0.f; });
+    over = wave_sum(over);
+    if (lane == 0) s_valid[w] = over;
     __syncthreads();
-    if (s_n <= SHORT) {
+    over = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) over += s_valid[i];
+    if (over <= SHORT) {
+      each([&](float x, int j) {
+        if (x >= least && kept(x, j)) list[atomicAdd(&s_n, 1u)].x = comp_of(x, j);
+      });
+      __syncthreads();
       draw_from_list(~0u, 1.f);
       return;
     }
   }
-
-  // what is left, in index order
   u64 sum = 0;
   again([&](float x, int j) {
     if (kept(x, j)) sum += weight(x);
@@ -478,32 +517,42 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   u64 total = 0, before = 0;
   for (int i = 0; i < NW; ++i) { if (i < w) before += red_a[i]; total += red_a[i]; }
   const double goal = (double)uu * (double)total;
-  if (sum && (double)before <= goal && (double)(before + sum) > goal) {       // one wave: the running sums rise
-    u64 base = before;
-    for (int s0 = j0; s0 < j1; s0 += 64) {
-      const int j = s0 + lane;
-      const float x = j < j1 ? load_logit(row, j) : -INFINITY;
-      const bool in = j < j1 && kept(x, j);
-      if (!__ballot(in)) continue;
-      u64 c = in ? weight(x) : 0;
-      const u64 own = c;
-      c = wave_scan_u64(c);
-      const u64 hit = __ballot(own && (double)(base + c) > goal);
-      if (hit) {
-        if (lane == __builtin_ctzll(hit)) {
-          a.token[b] = j;
-          a.logp[b] = logp_of(x, total);
-        }
-        break;
-      }
-      base += lane_u64(c, 63);
+  if (lane == 0 && sum && (double)before <= goal && (double)(before + sum) > goal) { s_bin = w; s_base = before; }       // one wave: the running sums rise
+  __syncthreads();
+  // its part again, by all threads: a run of neighbouring entries each
+  const int p0 = min(V, (int)s_bin * seg), p1 = min(V, p0 + seg), run = (p1 - p0 + NT - 1) / NT, r0 = min(p1, p0 + tid * run), r1 = min(p1, r0 + run);
+  u64 own = 0, first[4] = {0, 0, 0, 0};                  // (the weights of the run's first four, for the walk below)
+  for (int j = r0; j < r1; j += 4) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = load_logit(row, min(j + i, V - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u64 v = j + i < r1 && kept(x[i], j + i) ? weight(x[i]) : 0;
+      if (j == r0) first[i] = v;
+      own += v;
     }
   }
+  u64 c = wave_scan_u64(own);
+  if (lane == 63) red_b[w] = c;
+  __syncthreads();
+  c += s_base - own;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) c += i < w ? red_b[i] : 0;
+  if (own && (double)c <= goal && (double)(c + own) > goal)
+    for (int j = r0; j < r1; ++j) {
+      const int i = j - r0;
+      u64 v = i == 0 ? first[0] : i == 1 ? first[1] : i == 2 ? first[2] : first[3];
+      if (i > 3) { const float x = load_logit(row, j); v = kept(x, j) ? weight(x) : 0; }
+      c += v;
+      if ((double)c > goal) { a.token[b] = j; a.logp[b] = logp_of(load_logit(row, j), total); break; }
+    }
 }
 
 template <typename T> void launch(const SampleArgs& a, int B, hipStream_t st) {
   if (a.V <= 256) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 1>), dim3(B), dim3(256), 0, st, a);
   else if (a.V <= 4096) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 16>), dim3(B), dim3(256), 0, st, a);
+  else if (a.V <= 8192) hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 8>), dim3(B), dim3(1024), 0, st, a);
   else if (a.V <= 32768) hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 32>), dim3(B), dim3(1024), 0, st, a);
   else hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 0>), dim3(B), dim3(1024), 0, st, a);
 }

@@ -364,7 +364,7 @@ int dsrg_action_tail_fwd(const float* logits, int ld, const int64_t* targets, in
  * top_k, top_p and min_p: fp32 / int32 device arrays [B], or NULL for the number beside them.  The candidates in falling order
  * (equal values: the lowest index first) are cut (1) after the k-th (k <= 0: no cut); (2) after the first whose running sum of
  * weights w = exp((x - max) / T) reaches p of the sum over what (1) left (p >= 1: no cut; the first one always stays); (3) before
- * the first with w < m (m <= 0: no cut).  token[b] = the first entry, in index order, at which the running sum over what is left
+ * the first with w < m (m <= 0: no cut; m > 1: as 1).  token[b] = the first entry, in index order, at which the running sum over what is left
  * exceeds u[b] times the whole; logp[b] = its log-probability among them.  T <= 0 (or NaN): the largest entry, logp 0.  A row without
  * a candidate: token -1, logp -inf.  1 <= V <= 524288.  Deterministic: sums are 64-bit integers. */
 int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature, float temperature0,
@@ -401,7 +401,7 @@ int dsrg_kv_read(const dsrg_kv_cache_t* cache, void* k, int64_t k_bs, int k_rs, 
  * stands at position p = lens[b] - Nq + i (the Nq rows are the newest tokens, already in the cache) and sees t <= p, with window > 0
  * only t > p - window.  lens is clamped to the table's reach.  Rows that see nothing: o = 0, lse = -inf.  lse fp32 [B,nh,Nq] or
  * NULL: log-sum-exp of the scaled scores.  Scores, sums and O are held in fp32; bf16 / 8-bit caches round P (times the value's
- * scale) to bf16 for the matrix instruction.  Few rows: the tokens are split over workgroups and joined by a second kernel, through a
+ * scale) to two bf16 numbers for the matrix instruction.  Few rows: the tokens are split over workgroups and joined by a second kernel, through a
  * workspace of dsrg_attention_paged_workspace() bytes (0: none needed; negative: an error code) that belongs to this call until
  * it has run: two calls that may overlap need two. */
 int64_t dsrg_attention_paged_workspace(const dsrg_kv_cache_t* cache, int width, int B, int nh, int Nq, int window);

@@ -457,6 +457,29 @@ def test_sample_rows_masks_and_special_values(K):
     _check_rows(K, x, hi)
 
 
+@pytest.mark.parametrize('V', [40, 3000, 20000, 70000])
+def test_sample_rows_min_p_alone_and_parameters_out_of_range(K, V):
+    """min-p without the other cuts (few and many entries left); tensors may hold what a number may not: min-p over 1 (the largest alone), NaN and
+    negative values (no cut; temperature: the largest), top-p of 0 and below, top-k over the row"""
+    B = 8
+    logits = (torch.randn(B, V, generator=_g(V)) * 1.5).cuda()
+    u = torch.rand(B, generator=_g(1)).cuda()
+    for m in (0.9, 0.3, 0.01, 1e-5):
+        _check_rows(K, logits, u, 0.9, 0, 1.0, m)
+    t = lambda *v: torch.tensor(v, device='cuda')        # noqa: E731
+    nan = float('nan')
+    T = t(1.0, 1.0, nan, -1.0, 0.7, 0.7, 2.0, 0.7)
+    k = t(0, V + 5, 3, 3, -4, 300, 700, 2000).int()
+    p = t(0.5, -0.5, 0.9, 0.9, nan, 0.0, 0.8, 0.9)
+    m = t(1.7, 0.0, 0.1, 0.1, nan, 0.2, -1.0, 5.0)
+    tok, lp = K.sample_rows(logits, u, T, k, p, m)
+    for b in range(B):
+        pb, mb = p[b].item(), m[b].item()
+        rt, rl, _ = _sample_ref(logits[b], u[b].item(), T[b].item(), k[b].item(), 1.0 if pb != pb else pb, 0.0 if mb != mb else mb)
+        assert tok[b].item() == rt, b
+        assert abs(lp[b].item() - rl) <= abs(rl) * 2.0 ** -23 + V * 2.0 ** -44 + 1e-12, b
+
+
 def test_sample_rows_strided_rows(K):
     big = torch.randn(5, 1000, generator=_g(4)).cuda()
     u = torch.rand(5, generator=_g(5)).cuda()
