@@ -166,17 +166,23 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(const AppendArgs a
   const int in_page = (int)pos0 & (a.c.S - 1);
   const int v0 = (int)max(lo - pos0, 0ll), v1 = (int)min(hi - pos0, 32ll);          // the block's rows that the call writes
   const int d0 = (tid % LPR) * 8;
+  float x[2][32 / RPP][8];
+#pragma unroll
+  for (int which = 0; which < 2; ++which)              // (every load of the block first)
+#pragma unroll
+    for (int q = 0; q < 32 / RPP; ++q) {
+      const int r = q * RPP + tid / LPR;
+      const TI* src = (const TI*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (pos0 + min(max(r, v0), v1 - 1) - start) * (which ? a.v_rs : a.k_rs) + h * D + d0;
+      ld8(src, x[which][q]);
+    }
 #pragma unroll
   for (int which = 0; which < 2; ++which)
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += RPP) {
-      const int r = r0 + tid / LPR;
+    for (int q = 0; q < 32 / RPP; ++q) {
+      const int r = q * RPP + tid / LPR;
       if (r < v0 || r >= v1) continue;
-      const TI* src = (const TI*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + (pos0 + r - start) * (which ? a.v_rs : a.k_rs) + h * D + d0;
-      float x[8];
-      ld8(src, x);
       TS w[8];
-      encode<KV, D>(x, w, d0, (which ? a.c.vs : a.c.ks), ph * a.c.S + in_page + r);
+      encode<KV, D>(x[which][q], w, d0, (which ? a.c.vs : a.c.ks), ph * a.c.S + in_page + r);
       if (which == 0) {
 #pragma unroll
         for (int j = 0; j < 8; j += E) __builtin_memcpy(__builtin_assume_aligned(sk + k_off<KV, D>(r, d0 + j), E * SZ), &w[j], E * SZ);
@@ -218,7 +224,7 @@ template <int KV, int D, typename TO>
 __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
   typedef typename KvT<KV>::type TS;
   typedef VTile<KV, D> VT;
-  constexpr int LPR = D / 8, RPP = 256 / LPR, E = KvT<KV>::E, SZ = KvT<KV>::SZ;
+  constexpr int LPR = D / 8, RPP = 256 / LPR, E = KvT<KV>::E, SZ = KvT<KV>::SZ;       // (RPP rows at a time: all 32, or 16)
   __shared__ __attribute__((aligned(16))) TS sv[VT::SIZE];
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const long long start = a.start ? a.start[b] : 0, pos0 = (start & ~31ll) + 32ll * blockIdx.x;
@@ -228,41 +234,41 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
   if (pos0 >= 0 && pos0 < (long long)a.width * a.c.S && pos0 - start < count) page = a.table[(long long)b * a.table_ld + (pos0 >> a.c.lgS)];
   const bool there = page >= 0 && page < a.c.P;
   const long long ph = (long long)page * a.c.H + h, row0 = ph * a.c.S + ((int)pos0 & (a.c.S - 1));
-  if (there) {
-    const TS* vs = (const TS*)a.c.v + row0 * D;
+  const int d0 = (tid % LPR) * 8;
+  TS ek[32 / RPP][8];
+  float sc[2][32 / RPP];
+  if (there) {                                          // (every load of the block first)
+    const TS *ks = (const TS*)a.c.k + row0 * D, *vs = (const TS*)a.c.v + row0 * D;
+    TS ev[32 * D / E / 256][E];
 #pragma unroll
-    for (int q0 = 0; q0 < 32 * D / E; q0 += 256) {
-      const int q = q0 + tid;
-      __builtin_memcpy(__builtin_assume_aligned(sv + VT::at(q * E), E * SZ), __builtin_assume_aligned(vs + q * E, E * SZ), E * SZ);
+    for (int q = 0; q < 32 * D / E / 256; ++q) __builtin_memcpy(ev[q], __builtin_assume_aligned(vs + (q * 256 + tid) * E, E * SZ), E * SZ);
+#pragma unroll
+    for (int q = 0; q < 32 / RPP; ++q) {
+      const int r = q * RPP + tid / LPR;
+#pragma unroll
+      for (int j = 0; j < 8; j += E) __builtin_memcpy(&ek[q][j], __builtin_assume_aligned(ks + k_off<KV, D>(r, d0 + j), E * SZ), E * SZ);
+      if constexpr (SZ == 1) { sc[0][q] = a.c.ks[row0 + r]; sc[1][q] = a.c.vs[row0 + r]; }
     }
+#pragma unroll
+    for (int q = 0; q < 32 * D / E / 256; ++q) __builtin_memcpy(__builtin_assume_aligned(sv + VT::at((q * 256 + tid) * E), E * SZ), ev[q], E * SZ);
     __syncthreads();
   }
-  const int d0 = (tid % LPR) * 8;
 #pragma unroll
   for (int which = 0; which < 2; ++which)
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += RPP) {
-      const int r = r0 + tid / LPR;
+    for (int q = 0; q < 32 / RPP; ++q) {
+      const int r = q * RPP + tid / LPR;
       const long long t = pos0 + r - start;
       if (t < 0 || t >= a.N) continue;
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = 0.f;
       if (there && t < count) {
-        TS e[8];
-        if (which == 0) {
-          const TS* ks = (const TS*)a.c.k + row0 * D;
-#pragma unroll
-          for (int j = 0; j < 8; j += E) __builtin_memcpy(&e[j], __builtin_assume_aligned(ks + k_off<KV, D>(r, d0 + j), E * SZ), E * SZ);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = sv[VT::at(v_off<KV, D>(r, d0 + j))];
-        }
-        const float s = SZ == 1 ? (which ? a.c.vs : a.c.ks)[row0 + r] : 1.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if constexpr (SZ == 1) x[j] = kv_value<KV>(e[j]) * s;
-          else x[j] = Elem<TS>::ld(&e[j]);
+          const TS e = which ? sv[VT::at(v_off<KV, D>(r, d0 + j))] : ek[q][j];
+          if constexpr (SZ == 1) x[j] = kv_value<KV>(e) * sc[which][q];
+          else x[j] = Elem<TS>::ld(&e);
         }
       }
       TO* dst = (TO*)(which ? a.v : a.k) + b * (which ? a.v_bs : a.k_bs) + t * (which ? a.v_rs : a.k_rs) + h * D + d0;
