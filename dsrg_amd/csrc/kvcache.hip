@@ -165,6 +165,7 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(const AppendArgs a
   const long long ph = (long long)page * a.c.H + h;
   const int in_page = (int)pos0 & (a.c.S - 1);
   const int v0 = (int)max(lo - pos0, 0ll), v1 = (int)min(hi - pos0, 32ll);          // the block's rows that the call writes
+  if (v0 >= v1) return;                                                              // (a sequence with nothing to write may start inside a block)
   const int d0 = (tid % LPR) * 8;
   float x[2][32 / RPP][8];
 #pragma unroll
@@ -742,8 +743,9 @@ int check_cache(const dsrg_kv_cache_t* c, const char* who, Pool& p) {
   p = Pool{c->k_pool, c->v_pool, c->k_scale, c->v_scale, c->n_pages, c->page_size, lg, c->n_kv_heads};
   return DSRG_OK;
 }
+constexpr long long MAX_TOKENS = 1ll << 30;       // that a table reaches: positions and their differences fit 32 bits
 int check_table(const char* who, const int32_t* table, int ld, int width, int S, int B) {
-  DSRG_CHECK(table && width >= 1 && (ld >= width || B <= 1) && (long long)width * S <= 0x7fffff00ll, "%s: bad page table (width %d, stride %d)", who, width, ld);
+  DSRG_CHECK(table && width >= 1 && (ld >= width || B <= 1) && (long long)width * S <= MAX_TOKENS, "%s: bad page table (width %d, stride %d)", who, width, ld);
   return DSRG_OK;
 }
 bool rows16(const void* p, long long bs, long long rs, int size) { return (uintptr_t)p % 16 == 0 && bs * size % 16 == 0 && rs * size % 16 == 0; }
@@ -764,7 +766,7 @@ Split plan_split(int kv, int D, int ct, int B, int H, int cgs, long long max_tok
 }
 long long seen_tokens(int width, int S, int Nq, int window) {
   const long long cap = (long long)width * S;
-  if (!window) return cap;
+  if (!window || window >= cap) return cap;
   const long long w = (long long)window + Nq - 1 + 31;       // the first block may start up to 31 tokens early
   return w < cap ? w : cap;
 }
@@ -856,7 +858,7 @@ extern "C" int64_t dsrg_attention_paged_workspace(const dsrg_kv_cache_t* cache, 
   Pool p;
   const int rc = check_cache(cache, "dsrg_attention_paged_workspace", p);
   if (rc) return rc;
-  DSRG_CHECK(width >= 1 && B >= 0 && nh >= 1 && nh % p.H == 0 && Nq >= 0 && window >= 0 && (long long)width * p.S <= 0x7fffff00ll, "dsrg_attention_paged_workspace: bad arguments");
+  DSRG_CHECK(width >= 1 && B >= 0 && nh >= 1 && nh % p.H == 0 && Nq >= 0 && window >= 0 && (long long)width * p.S <= MAX_TOKENS, "dsrg_attention_paged_workspace: bad arguments");
   if (B == 0 || Nq == 0) return 0;
   const long long NC = (long long)Nq * (nh / p.H);
   DSRG_CHECK(NC <= (1 << 20), "dsrg_attention_paged_workspace: %lld query rows per key / value head", NC);
@@ -890,7 +892,7 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const Split s = plan_split(cache->dtype, D_, ct, B, a.c.H, cgs, seen_tokens(width, a.c.S, Nq, window));
   a.q = q; a.o = o; a.lse = lse; a.q_bs = q_bs; a.o_bs = o_bs; a.q_rs = q_rs; a.o_rs = o_rs;
   a.table = table; a.lens = lens; a.table_ld = table_ld; a.width = width; a.B = B; a.nh = nh; a.Nq = Nq;
-  a.causal = causal != 0; a.window = window; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
+  a.causal = causal != 0; a.window = window < (long long)width * a.c.S ? window : 0; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
   a.ws_o = (float*)workspace;
   a.ws_ml = need ? (float2*)((float*)workspace + (int64_t)B * a.c.H * a.NC * s.nsplit * D_) : nullptr;
   const dim3 grid(s.nsplit, a.c.H * cgs, B);

@@ -85,7 +85,7 @@ def test_append_layout_and_read(K, dtype, H, D, S):
     table = _table(B, width, P, 1)
     before = [None if t is None else t.view(torch.uint8).clone() for t in c.values()]
     want = {}
-    start, count = [0, 7, 19, width * S - 20], [45, 0, 31, 45]      # the last one runs past its table: 20 rows fit
+    start, count = [0, 7, 19, width * S - 20], [45, 0, 31, 45]      # the second writes nothing, from inside a block; the last one runs past its table: 20 rows fit
     for call in range(2):
         g = _g(10 + call)
         packed = torch.randn(B, T, 2, H * D, generator=g) * torch.exp(torch.randn(B, T, 1, 1, generator=g))
@@ -259,6 +259,13 @@ def test_attention_paged(K, dtype, nh, H, D, Nq, causal, window):
     """lengths of zero and one, below, at and past tiles and pages, fewer tokens than rows; head layouts (own, shared, one, more rows than a
     tile's 16 columns); pools hold NaN wherever nothing was written"""
     _attend_case(K, dtype, 9, Nq, nh, H, D, 32, [0, 1, 2, 15, 31, 32, 33, 129, 300], causal, window)
+
+
+@pytest.mark.parametrize('dtype', [BF16, I8])
+def test_attention_paged_window_over_everything(K, dtype):
+    """windows at and past the table's reach are none at all"""
+    for window in (128, 4096, 2 ** 31 - 1):
+        _attend_case(K, dtype, 4, 5, 8, 2, 64, 32, [0, 3, 70, 96], True, window, seed=9)
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32, I8, E4M3])

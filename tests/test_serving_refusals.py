@@ -47,7 +47,8 @@ def test_append_and_read_refusals():
         assert f(dt=_lib.I8) == -1
         assert f(k=66) == -1 and b'aligned' in lib.dsrg_last_error()
         assert f(kr=129) == -1 and f(kb=4) == -1
-        assert f(width=1 << 27) == -1 and b'table' in lib.dsrg_last_error()
+        assert f(width=(1 << 25) + 1) == -1 and b'table' in lib.dsrg_last_error()
+        assert f(B=70000, T=8) == -1 if f is app else f(B=70000) == -1
     assert app(start=None) == -1 and read(count=None) == -1 and app(T=-3) == -1 and read(n=-3) == -1
 
 
