@@ -114,10 +114,19 @@ __device__ __forceinline__ u64 wave_scan_u64(u64 v) {
   return v;
 }
 
-template <typename T> __device__ __forceinline__ float load_logit(const T* row, int j) {
-  const float x = Elem<T>::ld(row + j) + 0.0f;          // (-0 + 0 = +0: the two zeros are one value)
-  return x != x ? -INFINITY : x;
-}
+// -0 + 0 = +0: the two zeros are one value; NaN is no candidate
+__device__ __forceinline__ float candidate(float x) { return fmaxf(x + 0.0f, -INFINITY); }
+template <typename T> __device__ __forceinline__ float load_logit(const T* row, int j) { return candidate(Elem<T>::ld(row + j)); }
+// A row through a buffer descriptor: one lane offset and a scalar one serve all of a wave's loads, and what lies past the row reads as 0
+// without a comparison a load
+template <typename T> struct RowBuffer {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ RowBuffer(const T* row, int V) : r(__builtin_amdgcn_make_buffer_rsrc((void*)row, 0, V * (int)sizeof(T), 0x00027000)) {}
+  __device__ __forceinline__ T raw(int lane_at, int scalar_at) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, lane_at * 4, scalar_at * 4, 0));
+    else return __builtin_amdgcn_raw_buffer_load_b16(r, lane_at * 2, scalar_at * 2, 0);
+  }
+};
 
 // Where the row is: VPT > 0: a thread holds VPT values of it in registers for the passes of the short way (top-k with a small k, short
 // rows); the long way, taken by the others, reads the row again from the cache, eight independent loads at a time.
@@ -132,11 +141,11 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   static_assert(NB >= LIST, "one word an entry");
   __shared__ u64 tab[1024];
   __shared__ u64 red_a[NW], red_b[NW];
-  __shared__ float s_max[NW], s_valid[NW];
+  __shared__ float s_max[NW];
   __shared__ double s_c2, s_tlogm;
   __shared__ u64 s_thr, s_base, s_bin_v;
   __shared__ unsigned s_bin, s_n;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x, V = a.V;
   const T* row = (const T*)a.logits + (long long)b * a.ld;
   const float Tm = a.temp ? a.temp[b] : a.temp0, P = a.topp ? a.topp[b] : a.topp0, M = a.minp ? a.minp[b] : a.minp0;
   const int Kk = a.topk ? a.topk[b] : a.topk0;
@@ -145,28 +154,35 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   const int seg = (V + NW * 64 - 1) / (NW * 64) * 64, j0 = min(V, w * seg), j1 = min(V, j0 + seg);
 
   // f(value, index) for this thread's share of the row; -inf stands for what is no candidate
+  const RowBuffer<T> buf(row, V);
   auto again = [&](auto&& f) {
-    for (int jb = j0 + lane; jb - lane < j1; jb += 512) {
-      float x[8];
+    for (int jb = j0; jb < j1; jb += 512) {
+      T x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = load_logit(row, min(jb + i * 64, V - 1));
+      for (int i = 0; i < 8; ++i) x[i] = buf.raw(lane, jb + i * 64);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f(jb + i * 64 < j1 ? x[i] : -INFINITY, jb + i * 64);
+      for (int i = 0; i < 8; ++i) f(jb + i * 64 + lane < j1 ? candidate(Elem<T>::ld(&x[i])) : -INFINITY, jb + i * 64 + lane);
+    }
+  };
+  auto constants = [&] {                                // (while the row is on its way)
+    for (int k = tid; k < 1024; k += NT) tab[k] = exp2_table(k);
+    if (tid == NT - 1) {
+      s_c2 = 1024 * 1.44269504088896340736 / (double)Tm;
+      s_tlogm = M > 0.f ? (double)Tm * log((double)M) : -INFINITY;
     }
   };
   float xs[VPT ? VPT : 1];
   if constexpr (VPT > 0) {
+    T x[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) xs[i] = load_logit(row, min(j0 + i * 64 + lane, V - 1));
+    for (int i = 0; i < VPT; ++i) x[i] = buf.raw(lane, j0 + i * 64);
+    constants();
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) xs[i] = j0 + i * 64 + lane < j1 ? xs[i] : -INFINITY;
-  }
-  // (while the row is on its way)
-  for (int k = tid; k < 1024; k += NT) tab[k] = exp2_table(k);
-  if (tid == NT - 1) {
-    s_c2 = 1024 * 1.44269504088896340736 / (double)Tm;
-    s_tlogm = M > 0.f ? (double)Tm * log((double)M) : -INFINITY;
-  }
+    for (int i = 0; i < VPT; ++i) {
+      xs[i] = candidate(Elem<T>::ld(&x[i]));
+      if (j0 + i * 64 + 64 > j1) xs[i] = j0 + i * 64 + lane < j1 ? xs[i] : -INFINITY;
+    }
+  } else constants();
   auto each = [&](auto&& f) {
     if constexpr (VPT > 0) {
 #pragma unroll
@@ -174,21 +190,16 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     } else again(f);
   };
 
-  // largest value, and how many entries can be drawn at all
+  // largest value
   float tmax = -INFINITY;
-  unsigned valid = 0;
-  each([&](float x, int) {
-    valid += x > -INFINITY;
-    tmax = fmaxf(tmax, x);
-  });
-  const float wmax = wave_max(tmax), wvalid = wave_sum((float)valid);
-  if (lane == 0) { s_max[w] = wmax; s_valid[w] = wvalid; }
+  each([&](float x, int) { tmax = fmaxf(tmax, x); });
+  const float wmax = wave_max(tmax);
+  if (lane == 0) s_max[w] = wmax;
   __syncthreads();
-  float mx = -INFINITY, fvalid = 0.f;                   // (counts up to 2^19: exact)
+  float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) { mx = fmaxf(mx, s_max[i]); fvalid += s_valid[i]; }
-  const int nvalid = (int)fvalid;
-  if (nvalid == 0) {                                    // nothing to draw from
+  for (int i = 0; i < NW; ++i) mx = fmaxf(mx, s_max[i]);
+  if (mx == -INFINITY) {                                // nothing to draw from
     if (tid == 0) { a.token[b] = -1; a.logp[b] = -INFINITY; }
     return;
   }
@@ -414,16 +425,27 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) total += red_b[i];
     const double draw = (double)uu * (double)total;
-    // (the low word is ~index: the entries before have a larger one)
-    ranked(n, [](const ulonglong2& o, const ulonglong2& me) { return (unsigned)o.x > (unsigned)me.x; }, [&](int, const ulonglong2& me, unsigned, u64 m) {
-      if (me.y && (double)m <= draw && (double)(m + me.y) > draw) { a.token[b] = (int)~(unsigned)me.x; a.logp[b] = logp_of(value(me.x), total); }
-    });
+    if constexpr (VPT == 1) {                           // the list is in index order, an entry a thread
+      const u64 own = tid < n ? list[tid].y : 0;
+      u64 c = wave_scan_u64(own);
+      if (lane == 63) red_a[w] = c;
+      __syncthreads();
+      c -= own;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) c += i < w ? red_a[i] : 0;
+      if (own && (double)c <= draw && (double)(c + own) > draw) { a.token[b] = (int)~(unsigned)list[tid].x; a.logp[b] = logp_of(value(list[tid].x), total); }
+    } else {
+      // (the low word is ~index: the entries before have a larger one)
+      ranked(n, [](const ulonglong2& o, const ulonglong2& me) { return (unsigned)o.x > (unsigned)me.x; }, [&](int, const ulonglong2& me, unsigned, u64 m) {
+        if (me.y && (double)m <= draw && (double)(m + me.y) > draw) { a.token[b] = (int)~(unsigned)me.x; a.logp[b] = logp_of(value(me.x), total); }
+      });
+    }
   };
 
   // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
   // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
   // wanted ones, and few others.  One bin a thread here (NT / 16 an octave): a bin costs a few more entries, a scan more costs time.
-  const bool small = VPT == 1, few = Kk > 0 && Kk <= 256 && Kk < nvalid;
+  const bool small = VPT == 1, few = Kk > 0 && Kk <= 256;
   if (small || few) {
     float lim = -3.4028235e38f;                         // entries from here on (every candidate: -inf and NaN are none)
     if (tid == 0) s_n = 0;
@@ -453,32 +475,59 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
         const double edge = __uint_as_float((last + lo + 1) << SN), at = (double)mx - edge * (1.0 + 0x1p-22);
         lim = fmaxf((float)(at - fabs(at) * 0x1p-22), lim);
       }
-    } else __syncthreads();
-    auto take = [&](float x, int j) {
-      if (x >= lim) {
-        const unsigned at = atomicAdd(&s_n, 1u);
-        if (at < LIST) list[at].x = comp_of(x, j);
-      }
-    };
-    if constexpr (VPT >= 8) {
+    }
+    if constexpr (VPT == 1) {                           // packed in index order
+      const bool in = xs[0] > -INFINITY;
+      const u64 hit = __ballot(in);
+      if (lane == 0) red_a[w] = __popcll(hit);
+      __syncthreads();
+      unsigned at = __popcll(hit & (((u64)1 << lane) - 1)), all = 0;
 #pragma unroll
-      for (int i = 0; i < VPT; i += 8) {                // (one test for eight: few of a wave's 512 are taken)
-        float m = xs[i];
+      for (int i = 0; i < NW; ++i) { at += i < w ? (unsigned)red_a[i] : 0u; all += (unsigned)red_a[i]; }
+      if (in) list[at].x = comp_of(xs[0], j0 + lane);
+      if (tid == 0) s_n = all;
+    } else {
+      auto take = [&](float x, int j) {
+        if (x >= lim) {
+          const unsigned at = atomicAdd(&s_n, 1u);
+          if (at < LIST) list[at].x = comp_of(x, j);
+        }
+      };
+      if constexpr (VPT >= 8) {
 #pragma unroll
-        for (int t = 1; t < 8; ++t) m = fmaxf(m, xs[i + t]);
-        if (__any(m >= lim))
+        for (int i = 0; i < VPT; i += 8) {                // (one test for eight: few of a wave's 512 are taken)
+          float m = xs[i];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) take(xs[i + t], j0 + (i + t) * 64 + lane);
-      }
-    } else each(take);
+          for (int t = 1; t < 8; ++t) m = fmaxf(m, xs[i + t]);
+          if (__any(m >= lim))
+#pragma unroll
+            for (int t = 0; t < 8; ++t) take(xs[i + t], j0 + (i + t) * 64 + lane);
+        }
+      } else each(take);
+    }
     __syncthreads();
-    if (s_n <= LIST) {
+    if (VPT == 1 || s_n <= LIST) {
       draw_from_list(Kk > 0 ? (unsigned)Kk : ~0u, P);
       return;
     }
     __syncthreads();
   }
-  if (Kk > 0 && Kk < nvalid) cut(false, (u64)Kk, 0.0);
+  // sum over the workgroup (of whole numbers below 2^24: exact)
+  auto count = [&](float v) {
+    __syncthreads();
+    v = wave_sum(v);
+    if (lane == 0) s_max[w] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += s_max[i];
+    return v;
+  };
+  if (Kk > 0) {
+    float n = 0.f;
+    each([&](float x, int) { n += x > -INFINITY ? 1.f : 0.f; });
+    if ((float)Kk < count(n)) cut(false, (u64)Kk, 0.0);
+  }
   if (P < 1.f) cut(true, 0, (double)P);
   auto kept = [&](float x, int j) { return x > -INFINITY && comp_of(x, j) >= thr && (x == mx || (double)x >= floor_); };
   __syncthreads();
@@ -492,12 +541,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     const float least = fminf(mx, fmaxf(thr ? of_key((unsigned)(thr >> 32)) : -3.4028235e38f, (float)(floor_ - fabs(floor_) * 0x1p-22)));
     float over = 0.f;
     each([&](float x, int) { over += x >= least ? 1.f : 0.f; });
-    over = wave_sum(over);
-    if (lane == 0) s_valid[w] = over;
-    __syncthreads();
-    over = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) over += s_valid[i];
+    over = count(over);
     if (over <= SHORT) {
       each([&](float x, int j) {
         if (x >= least && kept(x, j)) list[atomicAdd(&s_n, 1u)].x = comp_of(x, j);
