@@ -226,9 +226,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   };
 
   // For every entry of the list: what the entries weigh for which `ahead(other, me)` holds, and how many they are.  The 16 lanes of a DPP row
-  // share four entries and walk the list together.
+  // walk the list together for an entry (or two).
   auto ranked = [&](int n, auto&& ahead, auto&& f) {
-    constexpr int EB = 4;
+    constexpr int EB = NT == 1024 ? 1 : 2;
     const int sub = tid & 15;
     for (int i0 = 0; i0 < n; i0 += NT / 16 * EB) {
       const int i1 = i0 + (tid >> 4) * EB;
@@ -487,23 +487,36 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       if (in) list[at].x = comp_of(xs[0], j0 + lane);
       if (tid == 0) s_n = all;
     } else {
-      auto take = [&](float x, int j) {
-        if (x >= lim) {
-          const unsigned at = atomicAdd(&s_n, 1u);
-          if (at < LIST) list[at].x = comp_of(x, j);
+      if constexpr (VPT >= 8) {                         // counted first: one atomic a wave
+        unsigned mine = 0;
+        each([&](float x, int) { mine += x >= lim; });
+        const unsigned upto = wave_scan_u32(mine), total = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+        if (total) {
+          unsigned at = 0;
+          if (lane == 0) at = atomicAdd(&s_n, total);
+          at = (unsigned)__builtin_amdgcn_readfirstlane((int)at) + upto - mine;
+#pragma unroll
+          for (int i = 0; i < VPT; i += 8) {            // (one test for eight: few of a wave's 512 are taken)
+            float m = xs[i];
+#pragma unroll
+            for (int t = 1; t < 8; ++t) m = fmaxf(m, xs[i + t]);
+            if (__any(m >= lim))
+#pragma unroll
+              for (int t = 0; t < 8; ++t)
+                if (xs[i + t] >= lim) {
+                  if (at < LIST) list[at].x = comp_of(xs[i + t], j0 + (i + t) * 64 + lane);
+                  ++at;
+                }
+          }
         }
-      };
-      if constexpr (VPT >= 8) {
-#pragma unroll
-        for (int i = 0; i < VPT; i += 8) {                // (one test for eight: few of a wave's 512 are taken)
-          float m = xs[i];
-#pragma unroll
-          for (int t = 1; t < 8; ++t) m = fmaxf(m, xs[i + t]);
-          if (__any(m >= lim))
-#pragma unroll
-            for (int t = 0; t < 8; ++t) take(xs[i + t], j0 + (i + t) * 64 + lane);
-        }
-      } else each(take);
+      } else {
+        each([&](float x, int j) {
+          if (x >= lim) {
+            const unsigned at = atomicAdd(&s_n, 1u);
+            if (at < LIST) list[at].x = comp_of(x, j);
+          }
+        });
+      }
     }
     __syncthreads();
     if (VPT == 1 || s_n <= LIST) {
