@@ -14,7 +14,6 @@ typedef unsigned long long u64;
 
 namespace {
 
-constexpr int LIST = 1024;           // entries of the cut's bin that are ranked directly
 constexpr int WBITS = 44;
 
 struct SampleArgs {
@@ -135,6 +134,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   constexpr int NW = NT / 64, BPT = NB / NT;            // bins per thread
   __shared__ u64 mass[NB];
   __shared__ unsigned cnt[NB];
+  // Ranks cost n^2 / NT: entries of a cut's bin that are ranked directly (more: by the bits of their values), candidates of the short way, the
+  // k that goes there, and what a long way's end ranks.
+  constexpr int LIST = NT == 1024 ? 512 : 256, FEW = 3 * NT / 8, SHORT = NT / 4;
   __shared__ ulonglong2 list[LIST];                     // (comp, weight)
   u64* const l_ahead = mass;                            // (the short way has no use for the bins' weights)
   unsigned* const l_rank = cnt;
@@ -442,10 +444,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     }
   };
 
-  // The short way: everything that can be drawn fits a list.  Rows of up to 256 entries: all of them.  Top-k with a small k: the k-th
-  // largest of the threads' largest entries is no larger than the k-th largest of all, so the entries of its bin and above hold the k
-  // wanted ones, and few others.  One bin a thread here (NT / 16 an octave): a bin costs a few more entries, a scan more costs time.
-  const bool small = VPT == 1, few = Kk > 0 && Kk <= 256;
+  // The short way: everything that can be drawn fits a list.  Short rows: all of them (measured, 64 rows with top-p: V = 100 6.9 us against 8.8
+  // the long way, 170 the same, 256 12.1 against 9.3).  Top-k with a small k: the k-th largest of the threads' largest entries is no larger
+  // than the k-th largest of all, so the entries of its bin and above hold the k wanted ones, and few others (256 rows of 30522: k = 60 11.7 us
+  // against 28.5, k = 256 25.5 against 34.8, k = 400 50.9 against 38.5).  One bin a thread here (NT / 16 an octave): coarser ones cost a few
+  // entries more, a longer scan more time.
+  const bool small = VPT == 1, few = Kk > 0 && Kk <= SHORT;
   if (small || few) {
     float lim = -3.4028235e38f;                         // entries from here on (every candidate: -inf and NaN are none)
     if (tid == 0) s_n = 0;
@@ -519,7 +523,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       }
     }
     __syncthreads();
-    if (VPT == 1 || s_n <= LIST) {
+    if (VPT == 1 || s_n <= FEW) {
       draw_from_list(Kk > 0 ? (unsigned)Kk : ~0u, P);
       return;
     }
@@ -546,7 +550,6 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   __syncthreads();
 
   // what is left, in index order: each wave's part is summed; little of it in all is drawn from a list
-  constexpr unsigned SHORT = NT / 4;                    // (ranks cost n^2 / NT)
   if (thr || M > 0.f) {
     if (tid == 0) s_n = 0;
     __syncthreads();
@@ -607,7 +610,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
 }
 
 template <typename T> void launch(const SampleArgs& a, int B, hipStream_t st) {
-  if (a.V <= 256) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 1>), dim3(B), dim3(256), 0, st, a);
+  if (a.V <= 160) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 1>), dim3(B), dim3(256), 0, st, a);
   else if (a.V <= 4096) hipLaunchKernelGGL((sample_rows_kernel<T, 256, 1024, 16>), dim3(B), dim3(256), 0, st, a);
   else if (a.V <= 8192) hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 8>), dim3(B), dim3(1024), 0, st, a);
   else if (a.V <= 32768) hipLaunchKernelGGL((sample_rows_kernel<T, 1024, 4096, 32>), dim3(B), dim3(1024), 0, st, a);
