@@ -738,9 +738,11 @@ bool rows16(const void* p, long long bs, long long rs, int size) { return (uintp
 
 struct Split { int nw, nsplit, bps; };
 // How many waves share a sequence's tokens (per key / value head and column group): as many as fill the chip's places (1024 SIMDs) about
-// once (more than fit would wait for a second round), each with 64 tokens at least; at most 16384 tokens a workgroup, so that one long sequence among short ones does not run alone for
-// long.  Waves of a workgroup are joined in LDS, workgroups by a second kernel (4 to 5 us more): large workgroups where four waves are
-// not enough, and splits only where one of them is not.
+// once (more than fit would wait for a second round), each with 64 tokens at least; at most 16384 tokens a workgroup, so that one long
+// sequence among short ones does not run alone for long.  Waves of a workgroup are joined in LDS, workgroups by a second kernel (4 to 5 us
+// more): large workgroups where four waves are not enough, and splits only where one of them is not.  (26 thousand tokens of one sequence, two
+// heads of 128: 51 workgroups of 8 waves 14.3 us, 102 of 4 17.4; 16 sequences of up to 999, 12 fp32 heads: one of 12 waves each 17.2 us, 5 of 4
+// waves and the join 18.6; 264 workgroups instead of 240 on 256 CUs: 101 us instead of 66 for three sequences of 60 thousand.)
 Split plan_split(int kv, int D, int ct, int B, int H, int cgs, long long max_tokens) {
   const long long blocks = std::max((max_tokens + 31) / 32, 1ll), have = (long long)B * H * cgs, places = 1024ll * resident(kv, D, ct), most = most_waves(kv, D, ct);
   const long long waves = std::max(std::min(places / have, (blocks + 1) / 2), 4ll);
@@ -883,11 +885,13 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   a.causal = causal != 0; a.window = window < (long long)width * a.c.S ? window : 0; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
   a.ws_o = (float*)workspace;
   a.ws_ml = need ? (float2*)((float*)workspace + (int64_t)B * a.c.H * a.NC * s.nsplit * D_) : nullptr;
+  const long long rows = (long long)B * a.c.H * a.NC;
+  DSRG_CHECK(rows < (1ll << 31), "dsrg_attention_paged: %lld query rows", rows);
   const dim3 grid(s.nsplit, a.c.H * cgs, B);
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
-        constexpr int MW = most_waves(KV, D, 1);
+    constexpr int MW = most_waves(KV, D, 1);
     const int lds = s.nw * std::min(16, a.NC) * (D + 6) * 4;
     if (ct == 2) {
       if (mix) launch_paged<KV, D, 2, 4, true>(a, grid, lds, st);
@@ -902,7 +906,6 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   }))
   DSRG_LAUNCH_CHECK("dsrg_attention_paged");
   if (s.nsplit > 1) {
-    const long long rows = (long long)B * a.c.H * a.NC;
     const dim3 jgrid((unsigned)((rows + 3) / 4));
     D_SWITCH(D_, {
       if (dtype == DSRG_F32) hipLaunchKernelGGL((attention_paged_join_kernel<D, float>), jgrid, dim3(256), 0, st, a);

@@ -306,6 +306,7 @@ def test_attention_paged_masked_values_may_be_anything(K, dtype):
     assert torch.equal(o[:4], o2[:4]) and torch.isfinite(o2).all()
     assert torch.isnan(o[4:, 0]).all()                                             # K's NaN: the head's whole row
     assert torch.equal(o[4:6, 1], o2[4:6, 1])
+    assert not torch.isfinite(o[5:, 0, 3]).any()
     assert torch.isnan(o[6:, 1, 1]).all() and torch.equal(o[6:, 1, 2:], o2[6:, 1, 2:]) and torch.equal(o[6:, 1, 0], o2[6:, 1, 0])
 
 
@@ -487,8 +488,12 @@ def test_sample_rows_min_p_alone_and_parameters_out_of_range(K, V):
         assert abs(lp[b].item() - rl) <= abs(rl) * 2.0 ** -23 + V * 2.0 ** -44 + 1e-12, b
 
 
-def test_sample_rows_strided_rows(K):
-    big = torch.randn(5, 1000, generator=_g(4)).cuda()
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_sample_rows_strided_rows(K, dtype):
+    """rows that begin anywhere, and end anywhere in front of numbers that are larger than any of theirs"""
+    big = torch.randn(5, 1000, generator=_g(4))
+    big[:, :3] = big[:, 903:] = 50
+    big = big.to(dtype).cuda()
     u = torch.rand(5, generator=_g(5)).cuda()
     a = _check_rows(K, big[:, 3:903], u, 0.9, 30, 0.9)
     assert torch.equal(a, K.sample_rows(big[:, 3:903].contiguous(), u, 0.9, 30, 0.9)[0])
