@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
 // by a second kernel.
 // Bound by HBM where there is enough to read: 32 sequences of 1000-32768 tokens, 64 / 8 heads of 128, bf16: 2.21 GB in 430 us (5.15 TB/s; a 4 GiB
 // copy moves 4.75); 3 of 40-60 thousand in e4m3: 317 MB in 65 us with the join.  64 of 1-2011 tokens, 12 heads of 64, int8: 105 MB in
-// 31 us, bound by the CU with the longest sequences.  One of 200 tokens: 4.3 us, the chain launch - length - page - keys - output.
+// 28 us, the longest first.  One of 200 tokens: 4.3 us, the chain launch - length - page - keys - output.
 struct PagedArgs {
   Pool c;
   const void* q; void* o; float* lse;
@@ -311,6 +311,7 @@ struct PagedArgs {
   const int32_t *table, *lens;
   int table_ld, width, B, nh, G, Nq, NC;       // NC = Nq * G columns per (sequence, key / value head)
   int causal, window, nsplit, bps;             // bps: 32-token blocks per split
+  int longest_first;
   float sl2;                                   // scale * log2(e)
   float* ws_o; float2* ws_ml;                  // [B, H, NC, nsplit, D], [B, H, NC, nsplit]
 };
@@ -325,7 +326,9 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-__device__ __forceinline__ bf16x8 codes_to_bf16(uint2 u, int kv) {
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+__device__ __forceinline__ bf16x8 codes_to_bf16(u32x2 u, int kv) {
   bf16x8 r;
   if (kv == DSRG_E4M3) {
     bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.x, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u.x, 1.0f, true);
@@ -362,8 +365,29 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
   float* const sm = so + NW * nc * OLD;
   float* const sl = sm + NW * nc;
   const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int sp = blockIdx.x, H = a.c.H, kh = blockIdx.y % H, cg = blockIdx.y / H, b = blockIdx.z;
-  const int cap = a.width * a.c.S;
+  const int cap = a.width * a.c.S, sp = blockIdx.x, H = a.c.H;
+  int y = blockIdx.y, b = blockIdx.z;
+  if (a.longest_first) {
+    // Several workgroups a CU and sequences of different lengths: the longest sequences' workgroups come first, every second round of 256 the
+    // other way round, so that a CU (workgroups go round the 256 in turn) gets long and short ones.  Every wave ranks lens for itself and gets
+    // the same answer; where none is long or all are alike that would only cost.  (64 x 12 heads of 64, int8, 1-2011 tokens: 33.2 -> 28.5 us;
+    // 64 x 8 heads of 128, bf16, 1-4000: 111 -> 96; all of 2011 tokens, ranked all the same: 43.5 -> 45.1.)
+    const int mine = lane < a.B ? min(max(a.lens[lane], 0), cap) : -1;
+    const float longest = wave_max((float)mine), shortest = -wave_max(lane < a.B ? -(float)mine : -INFINITY);
+    if (longest >= 1024.f && shortest < 0.5f * longest) {
+      const unsigned gy = gridDim.y, total = gy * gridDim.z;
+      unsigned at = y + gy * b;
+      if ((at & 256) && (at | 255) < total) at ^= 255;
+      y = at % gy;
+      int rank = 0;
+      for (int j = 0; j < a.B; ++j) {
+        const int o = __builtin_amdgcn_readlane(mine, j);
+        rank += o > mine || (o == mine && j < lane);
+      }
+      b = __builtin_ctzll(__ballot(lane < a.B && rank == (int)(at / gy)));
+    }
+  }
+  const int kh = y % H, cg = y / H;
   const int len = min(max(a.lens[b], 0), cap);
   const int lo_all = a.window ? max(0, len - a.Nq - a.window + 1) : 0;       // first token any row sees
   const int blk0 = lo_all >> 5, blk_end = (len + 31) >> 5;
@@ -372,7 +396,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 
   // queries and what each column sees: [lo, hi)
   int hi[CT], lo[CT];
-  using QF = typename std::conditional<F, float4, bf16x8>::type;
+  using QF = typename std::conditional<F, f32x4, bf16x8>::type;
   QF qf[CT][KS];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -384,9 +408,9 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
     const TQ* qp = (const TQ*)a.q + b * a.q_bs + (long long)i * a.q_rs + (long long)h * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      if constexpr (F) qf[ct][s] = live ? *reinterpret_cast<const float4*>(qp + 16 * s + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (F) qf[ct][s] = live ? *reinterpret_cast<const f32x4*>(qp + 16 * s + 4 * g) : f32x4{0.f, 0.f, 0.f, 0.f};
       else {
-        uint4 u = live ? *reinterpret_cast<const uint4*>(qp + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+        const u32x4 u = live ? *reinterpret_cast<const u32x4*>(qp + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
         qf[ct][s] = __builtin_bit_cast(bf16x8, u);
       }
     }
@@ -405,10 +429,12 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 
   const int32_t* trow = a.table + (long long)b * a.table_ld;
   const int lgB = a.c.lgS - 5, bmask = (1 << lgB) - 1;
-  using RF = typename std::conditional<F, float4, typename std::conditional<Q8, uint2, uint4>::type>::type;
+  // The compiler's own vectors, not HIP's float4 and uint4: those come apart into scalars that this compiler (ROCm 7.2) has put into registers
+  // of tuples that it took for dead (values' second to fourth elements overwritten before their products, in one instantiation for fp32).
+  using RF = typename std::conditional<F, f32x4, typename std::conditional<Q8, u32x2, u32x4>::type>::type;
   constexpr int E = KvT<KV>::E, VN = F ? 2 * DT : DT;
   RF kr[2][KS], vr[VN];
-  float4 ksc[2], vsc[2];
+  f32x4 ksc[2], vsc[2];
   // Where a step's block lies: its first row in the pools (times D: its elements).  A block on no page is read from page 0 and counts as
   // masked.
   struct Step { long long row0; bool there; };
@@ -427,14 +453,14 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
       for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const RF*>(kb + t * 16 * D + (s * 64 + lane) * E);
     if constexpr (Q8) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) ksc[t] = *reinterpret_cast<const float4*>(a.c.ks + st.row0 + 16 * t + 4 * g);
+      for (int t = 0; t < 2; ++t) ksc[t] = *reinterpret_cast<const f32x4*>(a.c.ks + st.row0 + 16 * t + 4 * g);
     }
   };
   auto load_v = [&](const Step& st) {
     const TS* vb = (const TS*)a.c.v + st.row0 * D;
     if constexpr (Q8) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) vsc[t] = *reinterpret_cast<const float4*>(a.c.vs + st.row0 + 16 * t + 4 * g);
+      for (int t = 0; t < 2; ++t) vsc[t] = *reinterpret_cast<const f32x4*>(a.c.vs + st.row0 + 16 * t + 4 * g);
     }
 #pragma unroll
     for (int dt = 0; dt < VN; ++dt) vr[dt] = *reinterpret_cast<const RF*>(vb + (dt * 64 + lane) * E);
@@ -456,13 +482,10 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         if constexpr (F) {
-          const float kf[4] = {kr[t][s].x, kr[t][s].y, kr[t][s].z, kr[t][s].w};
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            const float qq[4] = {qf[ct][s].x, qf[ct][s].y, qf[ct][s].z, qf[ct][s].w};
+          for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s_[ct][t], 0, 0, 0);
-          }
+            for (int j = 0; j < 4; ++j) s_[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[t][s][j], qf[ct][s][j], s_[ct][t], 0, 0, 0);
         } else {
           bf16x8 kf;
           if constexpr (Q8) kf = codes_to_bf16(kr[t][s], KV);
@@ -478,7 +501,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s_[ct][t][i] *= (&ksc[t].x)[i];
+          for (int i = 0; i < 4; ++i) s_[ct][t][i] *= ksc[t][i];
     }
     if (more) load_k(nxt);
 
@@ -521,7 +544,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
         l[ct] += (s_[ct][t][0] + s_[ct][t][1]) + (s_[ct][t][2] + s_[ct][t][3]);
         if constexpr (Q8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s_[ct][t][i] = (full || s_[ct][t][i] != 0.f) ? s_[ct][t][i] * (&vsc[t].x)[i] : 0.f;
+          for (int i = 0; i < 4; ++i) s_[ct][t][i] = (full || s_[ct][t][i] != 0.f) ? s_[ct][t][i] * vsc[t][i] : 0.f;
         }
       }
     }
@@ -537,16 +560,15 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
           const int key = key0 + (F ? 16 * (dt / DT) + j : 16 * (j >> 2) + (j & 3));
           const bool in = cur.there && key < len && key >= lo_all;
           if constexpr (F) {
-            float& x = (&vr[dt].x)[j];
-            x = in ? x : 0.f;
+            const float x = in ? vr[dt][j] : 0.f;
+            vr[dt][j] = x;
             if (MIX) odd = odd || !(fabsf(x) <= 3.4028235e38f);
           } else if constexpr (Q8) {
-            unsigned& x = j < 4 ? vr[dt].x : vr[dt].y;
-            x = in ? x : x & ~(0xffu << (8 * (j & 3)));
+            const unsigned x = vr[dt][j >> 2];
+            vr[dt][j >> 2] = in ? x : x & ~(0xffu << (8 * (j & 3)));
           } else {
-            unsigned& x = (&vr[dt].x)[j >> 1];
-            const unsigned half = j & 1 ? 0xffff0000u : 0x0000ffffu;
-            x = in ? x : x & ~half;
+            const unsigned half = j & 1 ? 0xffff0000u : 0x0000ffffu, x = in ? vr[dt][j >> 1] : vr[dt][j >> 1] & ~half;
+            vr[dt][j >> 1] = x;
             if (MIX) odd = odd || (x & half & 0x7f807f80u) == (half & 0x7f807f80u);
           }
         }
@@ -560,8 +582,8 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
           float x[E];
 #pragma unroll
           for (int j = 0; j < E; ++j) {
-            if constexpr (F) x[j] = (&vr[dt].x)[j];
-            else { const unsigned v = (&vr[dt].x)[j >> 1]; x[j] = __uint_as_float(j & 1 ? v & 0xffff0000u : v << 16); }
+            if constexpr (F) x[j] = vr[dt][j];
+            else { const unsigned v = vr[dt][j >> 1]; x[j] = __uint_as_float(j & 1 ? v & 0xffff0000u : v << 16); }
           }
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
@@ -585,8 +607,8 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
           for (int j = 0; j < E; ++j)
             if (!(fabsf(x[j]) <= 3.4028235e38f)) {
-              if constexpr (F) (&vr[dt].x)[j] = 0.f;
-              else (&vr[dt].x)[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+              if constexpr (F) vr[dt][j] = 0.f;
+              else vr[dt][j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
       }
@@ -599,7 +621,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32((&vr[t * DT + dt].x)[i], s_[ct][t][i], o[ct][dt], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[t * DT + dt][i], s_[ct][t][i], o[ct][dt], 0, 0, 0);
     } else {
       // P as the sum of two bf16 numbers (16 bits of it): the matrix units wait for memory, and one rounding of P to 8 bits would be as
       // large an error as the output's own
@@ -890,6 +912,7 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const dim3 grid(s.nsplit, a.c.H * cgs, B);
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
+  a.longest_first = s.nsplit == 1 && B > 1 && B <= 64 && a.c.H * cgs * B > 256 && !a.window && (long long)width * a.c.S >= 1024;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
     constexpr int MW = most_waves(KV, D, 1);
     const int lds = s.nw * std::min(16, a.NC) * (D + 6) * 4;

@@ -276,6 +276,18 @@ def test_attention_paged_split(K, dtype):
     _attend_case(K, dtype, 2, 1, 2, 1, 64, 128, [20000, 128], seed=5)
 
 
+@pytest.mark.parametrize('dtype,B,Nq,nh,H,D,causal', [(I8, 37, 1, 12, 12, 64, False), (BF16, 64, 2, 16, 8, 128, True), (F32, 2, 1, 160, 160, 64, False), (E4M3, 33, 1, 8, 8, 64, False)])
+def test_attention_paged_ragged_batches(K, dtype, B, Nq, nh, H, D, causal):
+    """more workgroups than CUs over sequences of very different lengths, which are taken longest first: equal lengths, empty ones and the longest in
+    any place, full and partial rounds of workgroups"""
+    lens = torch.randint(0, 1400, (B,), generator=_g(B)).tolist()
+    lens[-1] = 1500
+    lens[0] = 0
+    lens[B // 2:B // 2 + 5] = [700] * len(lens[B // 2:B // 2 + 5])
+    lens[-1] = 1500
+    _attend_case(K, dtype, B, Nq, nh, H, D, 64, lens, causal=causal, seed=B)
+
+
 def test_attention_paged_scales_and_large_scores(K):
     """scores of hundreds (one token takes the whole row), a scale of its own, a negative one"""
     _attend_case(K, BF16, 2, 2, 4, 2, 64, 32, [700, 90], seed=6, spread=8.0)
