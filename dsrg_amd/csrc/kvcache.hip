@@ -670,7 +670,8 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ww = 0; ww < NW; ++ww) {
-        const float mw = sm[ww * nc + c], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
+        // (a wave without a maximum: its sum is 0, or NaN where all that it saw were NaN)
+        const float mw = sm[ww * nc + c], f = mw == -INFINITY ? sl[ww * nc + c] : __builtin_amdgcn_exp2f(mw - M);
         if (f != 0.f) {
           L += f * sl[ww * nc + c];
           O += f * *reinterpret_cast<const f32x4*>(so + (ww * nc + c) * OLD + d);
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
         const int i = n / a.G, h = kh * a.G + n - i * a.G;
         const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);       // (a NaN sum stays one)
         st4((TQ*)a.o + b * a.o_bs + (long long)i * a.o_rs + (long long)h * D + d, make_float4(O[0] * inv, O[1] * inv, O[2] * inv, O[3] * inv));
-        if (a.lse && d == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = M == -INFINITY ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+        if (a.lse && d == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
       } else {
         const long long row = ((long long)b * H + kh) * a.NC + n;
         *reinterpret_cast<f32x4*>(a.ws_o + (row * a.nsplit + sp) * D + d) = O;
@@ -709,9 +710,9 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) O[j] = 0.f;
   for (int s0 = 0; s0 < ns; s0 += 64) {
-    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing); then 8 splits' partial sums at a time
+    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing; NaN for one that saw nothing else); then 8 splits' partial sums at a time
     const float2 v = s0 + lane < ns ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
-    const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
+    const float f = v.x == -INFINITY ? v.y : __builtin_amdgcn_exp2f(v.x - M);
     L += wave_sum(f == 0.f ? 0.f : f * v.y);
     const int cnt = min(64, ns - s0);
     for (int s = 0; s < cnt; s += 8) {
@@ -733,7 +734,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
   TQ* op = (TQ*)a.o + b * a.o_bs + (long long)i * a.o_rs + (long long)h * D;
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) Elem<TQ>::st(op + lane + 64 * j, O[j] * inv);
-  if (a.lse && lane == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = M == -INFINITY ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+  if (a.lse && lane == 0) a.lse[((long long)b * a.nh + h) * a.Nq + i] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------

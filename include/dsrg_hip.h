@@ -400,8 +400,8 @@ int dsrg_kv_read(const dsrg_kv_cache_t* cache, void* k, int64_t k_bs, int k_rs, 
  * q, o [B, Nq, nh * head_dim] in dtype (fp32 for an fp32 cache, else bf16).  A row sees the tokens t < lens[b]; with causal = 1 row i
  * stands at position p = lens[b] - Nq + i (the Nq rows are the newest tokens, already in the cache) and sees t <= p, with window > 0
  * only t > p - window.  lens is clamped to the table's reach.  Rows that see nothing: o = 0, lse = -inf.  What a row
- * does not see may be infinite or NaN; of what it sees, a value that is not finite gives an output that is not.  lse fp32 [B,nh,Nq] or
- * NULL: log-sum-exp of the scaled scores.  Scores, sums and O are held in fp32; bf16 / 8-bit caches round P (times the value's
+ * does not see may be infinite or NaN; of what it sees, a value that is not finite gives an output that is not, and a score that is NaN
+ * or +inf an o and lse of NaN (one of -inf weighs nothing).  lse fp32 [B,nh,Nq] or NULL: log-sum-exp of the scaled scores.  Scores, sums and O are held in fp32; bf16 / 8-bit caches round P (times the value's
  * scale) to two bf16 numbers for the matrix instruction.  Few rows: the tokens are split over workgroups and joined by a second kernel, through a
  * workspace of dsrg_attention_paged_workspace() bytes (0: none needed; negative: an error code) that belongs to this call until
  * it has run: two calls that may overlap need two. */

@@ -288,6 +288,37 @@ def test_attention_paged_ragged_batches(K, dtype, B, Nq, nh, H, D, causal):
     _attend_case(K, dtype, B, Nq, nh, H, D, 64, lens, causal=causal, seed=B)
 
 
+@pytest.mark.parametrize('dtype', [BF16, F32, I8, E4M3])
+@pytest.mark.parametrize('Nq,causal', [(1, False), (3, True)])
+def test_attention_paged_nan_scores_show(K, dtype, Nq, causal):
+    """a NaN among the scores that a row sees makes its o and lse NaN, also where a wave (a workgroup) saw nothing else; other heads, other
+    sequences and rows that do not see it stay as they are"""
+    nh, H, D, S, lens, at = 4, 2, 64, 32, [1, 40, 5000, 5000, 70], [0, 39, 4990, 3, None]
+    B, n, io = len(lens), max(lens), IO[dtype]
+    width = -(-n // S)
+    P = B * width + 1
+    c, table, L = _cache(K, P, S, H, D, dtype), _table(B, width, P, 1), _i(*lens)
+    x = torch.randn(B, n, 2, H * D, generator=_g(2)).to(io).cuda()
+    K.kv_append(x[:, :, 0], x[:, :, 1], table=table, start=torch.zeros_like(L), count=L, **c)
+    q = torch.randn(B, Nq, nh * D, generator=_g(3)).to(io).cuda()
+    q[4, Nq - 1, 3 * D + 5] = float('nan')            # one row's last head
+    for b, t in enumerate(at):
+        if t is None:
+            continue
+        k = x[b:b + 1, t:t + 1, 0].clone()
+        k[..., :D] = float('nan')                     # the first key / value head
+        K.kv_append(k, x[b:b + 1, t:t + 1, 1], table=table[b:b + 1], start=_i(t), **c)
+    o, lse = K.attention_paged(q, table=table, lens=L, nh=nh, causal=causal, want_lse=True, **c)
+    o = o.view(B, Nq, nh, D)
+    for b in range(B):
+        for i in range(Nq):
+            last = lens[b] - Nq + i if causal else lens[b] - 1
+            for h in range(nh):
+                bad = (at[b] is not None and h < nh // H and at[b] <= last) or (b == 4 and i == Nq - 1 and h == 3)
+                assert torch.isnan(o[b, i, h]).all() if bad else torch.isfinite(o[b, i, h]).all(), (b, i, h)
+                assert lse[b, h, i].isnan() if bad else (lse[b, h, i].isfinite() if last >= 0 else lse[b, h, i] == float('-inf')), (b, i, h)
+
+
 def test_attention_paged_scales_and_large_scores(K):
     """scores of hundreds (one token takes the whole row), a scale of its own, a negative one"""
     _attend_case(K, BF16, 2, 2, 4, 2, 64, 32, [700, 90], seed=6, spread=8.0)
@@ -498,6 +529,14 @@ def test_sample_rows_min_p_alone_and_parameters_out_of_range(K, V):
         rt, rl, _ = _sample_ref(logits[b], u[b].item(), T[b].item(), k[b].item(), 1.0 if pb != pb else pb, 0.0 if mb != mb else mb)
         assert tok[b].item() == rt, b
         assert abs(lp[b].item() - rl) <= abs(rl) * 2.0 ** -23 + V * 2.0 ** -44 + 1e-12, b
+
+
+@pytest.mark.parametrize('V', [40, 3000, 20000])
+def test_sample_rows_infinite_temperature(K, V):
+    """(a tensor may hold one; as a number it is refused) every candidate weighs the same, so min-p of 1 keeps them all"""
+    logits, u = torch.randn(4, V, generator=_g(V)).cuda(), torch.rand(4, generator=_g(2)).cuda()
+    for k, p, m in [(0, 1.0, 0.0), (0, 1.0, 1.0), (17, 1.0, 1.0), (0, 0.5, 1.0)]:
+        _check_rows(K, logits, u, torch.full((4,), float('inf'), device='cuda'), k, p, m)
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
