@@ -173,7 +173,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int k = tid; k < 1024; k += NT) tab[k] = exp2_table(k);
     if (tid == NT - 1) {
       s_c2 = 1024 * 1.44269504088896340736 / (double)Tm;
-      s_tlogm = M > 0.f ? (double)Tm * log((double)M) : -INFINITY;
+      s_tlogm = M > 0.f && Tm < INFINITY ? (double)Tm * log((double)M) : -INFINITY;      // (T infinite: all weigh 1)
     }
   };
   float xs[VPT ? VPT : 1];
