@@ -9,7 +9,7 @@
 // depend on the order of the atomics, and 2^-45 an entry is far below what a 24-bit random number resolves.
 // One workgroup a row.  Measured (fp32): 256 rows of 30522, k = 60, p = 0.92, m = 0.02: 14 us, of which the 31 MB take 5.3 (5.9 TB/s) and the
 // rest is one workgroup's chain of barriers; 64 rows of 100 with top-p: 5.4 us, the launch and the same chain; 64 rows of 30522 with
-// top-p alone 35 us and unfiltered 18 us, bound by the weights' instructions (one or two weights an entry, 29 instructions each) on 64 CUs.
+// top-p alone 36 us and unfiltered 17 us, bound by the weights' instructions (one or two weights an entry, 29 instructions each) on 64 CUs.
 #include "common.h"
 #include <math.h>
 
@@ -130,8 +130,9 @@ template <typename T> struct RowBuffer {
   }
 };
 
-// Where the row is: VPT > 0: a thread holds VPT values of it in registers for the passes of the short way (top-k with a small k, short
-// rows); the long way, taken by the others, reads the row again from the cache, eight independent loads at a time.
+// Where the row is: VPT > 0: a thread holds VPT values of it in registers (64 rows of 30522: unfiltered 18.3 -> 17.2 us, top-p 37.7 ->
+// 35.9 against reading them again); longer rows, and the passes that only crowded bins need, read the row from the cache, eight independent loads
+// at a time.
 template <typename T, int NT, int NB, int VPT>
 __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   constexpr int NW = NT / 64, BPT = NB / NT;            // bins per thread
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     clear(by_mass);
     if (tid == 0) { s_thr = ~0ull; s_n = 0; }
     __syncthreads();
-    again([&](float x, int j) {
+    each([&](float x, int j) {
       if (x > -INFINITY && comp_of(x, j) >= thr) put(by_mass, bin_of(x), x);
     });
     __syncthreads();
@@ -317,16 +318,41 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     const double slack = fabs((double)mx) * 0x1p-22, top = (double)mx - e0 * (1.0 - 0x1p-22) + slack, bottom = (double)mx - e1 * (1.0 + 0x1p-22) - slack;
     const float vtop = top < 3.4e38 ? (float)top : INFINITY, vbottom = bottom > -3.4e38 ? (float)bottom : -3.4028235e38f;
     const bool exact_only = !(fabs((double)mx) < 3e38);
-    {
+    // its parts: NB of equal width (the last bin, from 256 on: by the first bits of max - x)
+    const unsigned part_lo = (bin + BLO) << SH, part_sh = bin < NB - 1 ? SH - (NB == 4096 ? 12 : 10) : NB == 4096 ? 18 : 20;
+    auto part_of = [&](float x) -> unsigned {
+      const float d = x == mx ? 0.f : mx - x;
+      return bin ? (__float_as_uint(d) - part_lo) >> part_sh : (unsigned)(d * (NB * (NB == 4096 ? 255.f : 252.f)));      // (bin 0 ends at 2^-8 times 1 + 16 / NB)
+    };
+    int part = -1;                                        // (all of them)
+    auto gather = [&] {
       each([&](float x, int j) {
-        if ((exact_only ? x > -INFINITY : x >= vbottom && x <= vtop) && bin_of(x) == bin && comp_of(x, j) >= thr) {
+        if ((exact_only ? x > -INFINITY : x >= vbottom && x <= vtop) && bin_of(x) == bin && (part < 0 || part_of(x) == (unsigned)part) && comp_of(x, j) >= thr) {
           const unsigned at = atomicAdd(&s_n, 1u);
           if (at < LIST) list[at].x = comp_of(x, j);
         }
       });
       __syncthreads();
+      return (int)s_n;
+    };
+    int n = gather();
+    const u64 bin_base = base;
+    if (n > LIST) {
+      // more than are ranked: the same once more over the bin's parts (64 rows of 30522 entries of which the cut falls among 30 thousand within 0.01:
+      // 119 us without, 74 with; where they are all equal the way below is taken all the same: 147 and 184)
+      __syncthreads();
+      clear(by_mass);
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      again([&](float x, int j) {
+        if (x > -INFINITY && bin_of(x) == bin && comp_of(x, j) >= thr) put(by_mass, part_of(x), x);
+      });
+      __syncthreads();
+      locate(by_mass, want, frac, base, &goal);
+      part = (int)s_bin;
+      base = s_base;
+      n = gather();
     }
-    const int n = (int)s_n;
     if (n <= LIST) {
       for (int i = tid; i < n; i += NT) list[i].y = by_mass ? weight(of_key((unsigned)(list[i].x >> 32))) : 1;
       __syncthreads();
@@ -337,7 +363,9 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
       __syncthreads();
       thr = s_thr;
     } else {
-      // many entries in one bin (a flat row, or equal values): by the value's 32 bits, LB of them a pass
+      // still many (equal values): by the value's 32 bits, LB of them a pass
+      base = bin_base;
+      __syncthreads();
       constexpr int LB = NB == 4096 ? 12 : 10;
       unsigned prefix = 0, pmask = 0;
       for (int sh = 32; sh > 0;) {
@@ -571,7 +599,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     }
   }
   u64 sum = 0;
-  again([&](float x, int j) {
+  each([&](float x, int j) {
     if (kept(x, j)) sum += weight(x);
   });
   sum = wave_sum_u64(sum);

@@ -531,6 +531,19 @@ def test_sample_rows_min_p_alone_and_parameters_out_of_range(K, V):
         assert abs(lp[b].item() - rl) <= abs(rl) * 2.0 ** -23 + V * 2.0 ** -44 + 1e-12, b
 
 
+@pytest.mark.parametrize('V', [2000, 6000, 30522, 70000])
+@pytest.mark.parametrize('start,width,T', [(0.0, 0.003, 1.0), (0.0, 0.00397, 1.0), (5.0, 0.01, 1.0), (300.0, 90.0, 100.0), (700.0, 2.0, 1.0)])
+def test_sample_rows_crowded_bins(K, V, start, width, T):
+    """thousands of different values, and some equal ones, close together behind the largest: near it, in the middle, far away"""
+    B = 4
+    x = -(start + width * torch.rand(B, V, generator=_g(V)))
+    x[:, 5:40] = x[:, 50:51]
+    x[:, 77] = 0.0
+    logits, u = x.cuda(), torch.rand(B, generator=_g(3)).cuda()
+    for k, p, m in [(0, 0.7, 0.0), (V // 2, 1.0, 0.0), (V // 3, 0.4, 0.0), (0, 0.3, 1e-3)]:
+        _check_rows(K, logits, u, T, k, p, m)
+
+
 @pytest.mark.parametrize('V', [40, 3000, 20000])
 def test_sample_rows_infinite_temperature(K, V):
     """(a tensor may hold one; as a number it is refused) every candidate weighs the same, so min-p of 1 keeps them all"""
