@@ -12,6 +12,7 @@
 #include "common.h"
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -313,7 +314,6 @@ struct PagedArgs {
   const int32_t *table, *lens;
   int table_ld, width, B, nh, G, Nq, NC;       // NC = Nq * G columns per (sequence, key / value head)
   int causal, window, nsplit, bps;             // bps: 32-token blocks per split
-  int longest_first;
   float sl2;                                   // scale * log2(e)
   float* ws_o; float2* ws_ml;                  // [B, H, NC, nsplit, D], [B, H, NC, nsplit]
 };
@@ -353,7 +353,7 @@ constexpr int resident(int kv, int D, int CT) {
 }
 // Waves of a large workgroup (one column tile): all that a CU holds, so that a sequence's tokens are joined in LDS as far as that goes
 constexpr int most_waves(int kv, int D, int CT) { return CT > 1 ? 4 : 4 * resident(kv, D, 1); }
-template <int KV, int D, int CT, int NW, bool MIX>
+template <int KV, int D, int CT, int NW, bool MIX, bool LF>
 __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_kernel(const PagedArgs a) {
   typedef typename KvT<KV>::type TS;
   typedef typename std::conditional<KV == DSRG_F32, float, bf16_t>::type TQ;
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
   const int lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cap = a.width * a.c.S, sp = blockIdx.x, H = a.c.H;
   int y = blockIdx.y, b = blockIdx.z;
-  if (a.longest_first) {
+  if constexpr (LF) {
     // Several workgroups a CU and sequences of different lengths: the longest sequences' workgroups come first, every second round of 256 the
     // other way round, so that a CU (workgroups go round the 256 in turn) gets long and short ones.  Every wave ranks lens for itself and gets
     // the same answer; where none is long or all are alike that would only cost.  (64 x 12 heads of 64, int8, 1-2011 tokens: 33.2 -> 28.5 us;
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
     if (ct) __syncthreads();
     const float ls = col_sum(l[ct]);
     if (c16 < nv) {
-      if (g == 0) { sm[w * nc + c16] = m[ct]; sl[w * nc + c16] = ls; }
+      if (g == 0) { sm[w * nc + c16] = ls == ls ? m[ct] : ls; sl[w * nc + c16] = ls; }          // (all that it saw may be NaN: no maximum)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(so + (w * nc + c16) * OLD + dt * 16 + 4 * g) = o[ct][dt];
     }
@@ -672,8 +672,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ww = 0; ww < NW; ++ww) {
-        // (a wave without a maximum: its sum is 0, or NaN where all that it saw were NaN)
-        const float mw = sm[ww * nc + c], f = mw == -INFINITY ? sl[ww * nc + c] : __builtin_amdgcn_exp2f(mw - M);
+        const float mw = sm[ww * nc + c], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
         if (f != 0.f) {
           L += f * sl[ww * nc + c];
           O += f * *reinterpret_cast<const f32x4*>(so + (ww * nc + c) * OLD + d);
@@ -687,7 +686,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
       } else {
         const long long row = ((long long)b * H + kh) * a.NC + n;
         *reinterpret_cast<f32x4*>(a.ws_o + (row * a.nsplit + sp) * D + d) = O;
-        if (d == 0) a.ws_ml[row * a.nsplit + sp] = make_float2(M, L);
+        if (d == 0) a.ws_ml[row * a.nsplit + sp] = make_float2(L == L ? M : L, L);
       }
     }
   }
@@ -712,9 +711,9 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) O[j] = 0.f;
   for (int s0 = 0; s0 < ns; s0 += 64) {
-    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing; NaN for one that saw nothing else); then 8 splits' partial sums at a time
+    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing); then 8 splits' partial sums at a time
     const float2 v = s0 + lane < ns ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
-    const float f = v.x == -INFINITY ? v.y : __builtin_amdgcn_exp2f(v.x - M);
+    const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
     L += wave_sum(f == 0.f ? 0.f : f * v.y);
     const int cnt = min(64, ns - s0);
     for (int s = 0; s < cnt; s += 8) {
@@ -787,9 +786,9 @@ int col_tiles(int NC) { return NC > 16 ? 2 : 1; }
 
 }  // namespace
 
-template <int KV, int D, int CT, int NW, bool MIX> static void launch_paged(const PagedArgs& a, dim3 grid, int lds, hipStream_t st) {
-  if (NW * 16 * (D + 6) * 4 > 65536) DSRG_SET_MAX_LDS_ONCE((attention_paged_kernel<KV, D, CT, NW, MIX>), NW * 16 * (D + 6) * 4);
-  hipLaunchKernelGGL((attention_paged_kernel<KV, D, CT, NW, MIX>), grid, dim3(NW * 64), lds, st, a);
+template <int KV, int D, int CT, int NW, bool MIX, bool LF = false> static void launch_paged(const PagedArgs& a, dim3 grid, int lds, hipStream_t st) {
+  if (NW * 16 * (D + 6) * 4 > 65536) DSRG_SET_MAX_LDS_ONCE((attention_paged_kernel<KV, D, CT, NW, MIX, LF>), NW * 16 * (D + 6) * 4);
+  hipLaunchKernelGGL((attention_paged_kernel<KV, D, CT, NW, MIX, LF>), grid, dim3(NW * 64), lds, st, a);
 }
 
 #define KV_SWITCH(DT, ...)                                               \
@@ -915,17 +914,19 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const dim3 grid(s.nsplit, a.c.H * cgs, B);
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
-  a.longest_first = s.nsplit == 1 && B > 1 && B <= 64 && a.c.H * cgs * B > 256 && !a.window && (long long)width * a.c.S >= 1024;
+  // longest sequences first (in an instantiation of its own: it costs other calls 1 to 4 %): long sequences, several workgroups of four waves a CU
+  const bool lf = s.nsplit == 1 && s.nw == 4 && B > 1 && B <= 64 && a.c.H * cgs * B > 256 && !a.window && (long long)width * a.c.S >= 1024;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
     constexpr int MW = most_waves(KV, D, 1);
     const int lds = s.nw * std::min(16, a.NC) * (D + 6) * 4;
-    if (ct == 2) {
-      if (mix) launch_paged<KV, D, 2, 4, true>(a, grid, lds, st);
-      else launch_paged<KV, D, 2, 4, false>(a, grid, lds, st);
-    } else if (s.nw == 4) {
-      if (mix) launch_paged<KV, D, 1, 4, true>(a, grid, lds, st);
-      else launch_paged<KV, D, 1, 4, false>(a, grid, lds, st);
-    } else {
+    auto four = [&](auto tiles, auto mixed, auto first) { launch_paged<KV, D, decltype(tiles)::value, 4, decltype(mixed)::value, decltype(first)::value>(a, grid, lds, st); };
+    auto pick = [&](auto tiles) {
+      if (lf) mix ? four(tiles, std::true_type(), std::true_type()) : four(tiles, std::false_type(), std::true_type());
+      else mix ? four(tiles, std::true_type(), std::false_type()) : four(tiles, std::false_type(), std::false_type());
+    };
+    if (ct == 2) pick(std::integral_constant<int, 2>());
+    else if (s.nw == 4) pick(std::integral_constant<int, 1>());
+    else {
       if (mix) launch_paged<KV, D, 1, MW, true>(a, grid, lds, st);
       else launch_paged<KV, D, 1, MW, false>(a, grid, lds, st);
     }

@@ -276,7 +276,9 @@ def test_attention_paged_split(K, dtype):
     _attend_case(K, dtype, 2, 1, 2, 1, 64, 128, [20000, 128], seed=5)
 
 
-@pytest.mark.parametrize('dtype,B,Nq,nh,H,D,causal', [(I8, 37, 1, 12, 12, 64, False), (BF16, 64, 2, 16, 8, 128, True), (F32, 2, 1, 160, 160, 64, False), (E4M3, 33, 1, 8, 8, 64, False)])
+@pytest.mark.parametrize('dtype,B,Nq,nh,H,D,causal', [(I8, 37, 1, 12, 12, 64, False), (BF16, 64, 2, 16, 8, 128, True), (F32, 2, 1, 160, 160, 64, False), (E4M3, 33, 1, 8, 8, 64, False),
+                                                        (I8, 64, 1, 12, 12, 64, False), (F32, 8, 1, 80, 80, 64, False), (E4M3, 61, 3, 12, 12, 64, True), (BF16, 41, 9, 16, 8, 64, True),
+                                                        (F32, 33, 20, 8, 8, 128, False)])
 def test_attention_paged_ragged_batches(K, dtype, B, Nq, nh, H, D, causal):
     """more workgroups than CUs over sequences of very different lengths, which are taken longest first: equal lengths, empty ones and the longest in
     any place, full and partial rounds of workgroups"""
