@@ -321,6 +321,24 @@ def test_attention_paged_nan_scores_show(K, dtype, Nq, causal):
                 assert lse[b, h, i].isnan() if bad else (lse[b, h, i].isfinite() if last >= 0 else lse[b, h, i] == float('-inf')), (b, i, h)
 
 
+@pytest.mark.parametrize('dtype', [I8, E4M3])
+@pytest.mark.parametrize('nh', [2, 16])
+def test_attention_paged_hidden_rows_without_a_scale(K, dtype, nh):
+    """8-bit keys and values of a token that only the last row sees, written from NaN and infinities: the other rows do not notice"""
+    H, D, n = 2, 64, 40
+    x = torch.randn(1, n, 2, H * D, generator=_g(5)).to(BF16).cuda()
+    bad = x.clone()
+    bad[0, n - 1, :, 3], bad[0, n - 1, :, D + 7], bad[0, n - 1, :, D + 9] = float('nan'), float('inf'), float('-inf')
+    q = torch.randn(1, 3, nh * D, generator=_g(6)).to(BF16).cuda()
+    table, L, got = _i(2, 1)[None], _i(n), []
+    for rows in (x, bad):
+        c = _cache(K, 3, 32, H, D, dtype)
+        K.kv_append(rows[:, :, 0], rows[:, :, 1], table=table, start=_i(0), **c)
+        got.append(K.attention_paged(q, table=table, lens=L, nh=nh, causal=True, want_lse=True, **c))
+    assert torch.equal(got[0][0][:, :2], got[1][0][:, :2]) and torch.equal(got[0][1][..., :2], got[1][1][..., :2])
+    assert torch.isfinite(got[0][0]).all() and torch.isnan(got[1][0][:, 2]).all() and torch.isnan(got[1][1][..., 2]).all()
+
+
 def test_attention_paged_scales_and_large_scores(K):
     """scores of hundreds (one token takes the whole row), a scale of its own, a negative one"""
     _attend_case(K, BF16, 2, 2, 4, 2, 64, 32, [700, 90], seed=6, spread=8.0)
