@@ -119,14 +119,15 @@ __device__ __forceinline__ u64 wave_scan_u64(u64 v) {
 // -0 + 0 = +0: the two zeros are one value; NaN is no candidate
 __device__ __forceinline__ float candidate(float x) { return fmaxf(x + 0.0f, -INFINITY); }
 template <typename T> __device__ __forceinline__ float load_logit(const T* row, int j) { return candidate(Elem<T>::ld(row + j)); }
-// A row through a buffer descriptor: one lane offset and a scalar one serve all of a wave's loads, and what lies past the row reads as 0
-// without a comparison a load
+// A row through a buffer descriptor: what lies past the row is not read (it is 0) without a comparison a load.  The whole position goes into the
+// lane's offset, which is what the hardware compares with the row's size: a scalar offset is no certain part of that, and could pass the
+// size by itself.  One addition a load at most, neighbouring loads share theirs (constants fold into the instruction).
 template <typename T> struct RowBuffer {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ RowBuffer(const T* row, int V) : r(__builtin_amdgcn_make_buffer_rsrc((void*)row, 0, V * (int)sizeof(T), 0x00027000)) {}
-  __device__ __forceinline__ T raw(int lane_at, int scalar_at) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, lane_at * 4, scalar_at * 4, 0));
-    else return __builtin_amdgcn_raw_buffer_load_b16(r, lane_at * 2, scalar_at * 2, 0);
+  __device__ __forceinline__ T raw(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, j * 4, 0, 0));
+    else return __builtin_amdgcn_raw_buffer_load_b16(r, j * 2, 0, 0);
   }
 };
 
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int jb = j0; jb < j1; jb += 512) {
       T x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = buf.raw(lane, jb + i * 64);
+      for (int i = 0; i < 8; ++i) x[i] = buf.raw(jb + lane + i * 64);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f(jb + i * 64 + lane < j1 ? candidate(Elem<T>::ld(&x[i])) : -INFINITY, jb + i * 64 + lane);
     }
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
   if constexpr (VPT > 0) {
     T x[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) x[i] = buf.raw(lane, j0 + i * 64);
+    for (int i = 0; i < VPT; ++i) x[i] = buf.raw(j0 + lane + i * 64);
     constants();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
