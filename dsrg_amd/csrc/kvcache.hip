@@ -672,11 +672,10 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ww = 0; ww < NW; ++ww) {
+        // (a factor of 0 is multiplied too: an infinity or NaN among the values that a wave saw shows, whatever they weigh)
         const float mw = sm[ww * nc + c], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-        if (f != 0.f) {
-          L += f * sl[ww * nc + c];
-          O += f * *reinterpret_cast<const f32x4*>(so + (ww * nc + c) * OLD + d);
-        }
+        L += f * sl[ww * nc + c];
+        O += f * *reinterpret_cast<const f32x4*>(so + (ww * nc + c) * OLD + d);
       }
       if (a.nsplit == 1) {
         const int i = n / a.G, h = kh * a.G + n - i * a.G;
@@ -711,10 +710,11 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) O[j] = 0.f;
   for (int s0 = 0; s0 < ns; s0 += 64) {
-    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing); then 8 splits' partial sums at a time
+    // lane s has the factor of split s0 + s (0 past the end and for splits that saw nothing); then 8 splits' partial sums at a time, those with
+    // a factor of 0 as well (as above)
     const float2 v = s0 + lane < ns ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
     const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - M);
-    L += wave_sum(f == 0.f ? 0.f : f * v.y);
+    L += wave_sum(f * v.y);
     const int cnt = min(64, ns - s0);
     for (int s = 0; s < cnt; s += 8) {
       float p[8][D / 64];
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
       for (int t = 0; t < 8; ++t) {
         const float ft = s + t < cnt ? lane_f32(f, s + t) : 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) O[j] += ft == 0.f ? 0.f : ft * p[t][j];
+        for (int j = 0; j < D / 64; ++j) O[j] += s + t < cnt ? ft * p[t][j] : 0.f;
       }
     }
   }
