@@ -509,7 +509,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 
     const bool full = blk >= full_lo && blk < full_hi && cur.there;
     const int key0 = blk * 32 + 4 * g;
-    unsigned vis[CT];                      // MIX: a bit per score of the lane
+    unsigned vis[CT];                      // MIX and 8 bits: a bit per score of the lane, of a block that is not seen whole
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       vis[ct] = 0;
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
             const int key = key0 + 16 * t + i;
             const bool in = cur.there && key < hi[ct] && key >= lo[ct];
             s_[ct][t][i] = in ? s_[ct][t][i] * a.sl2 : -INFINITY;
-            if (MIX) vis[ct] |= in ? 1u << (4 * t + i) : 0u;
+            if (MIX || Q8) vis[ct] |= in ? 1u << (4 * t + i) : 0u;
           }
       } else {
 #pragma unroll
@@ -544,9 +544,9 @@ __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_
 #pragma unroll
         for (int i = 0; i < 4; ++i) s_[ct][t][i] = __builtin_amdgcn_exp2f(s_[ct][t][i] - mb);
         l[ct] += (s_[ct][t][0] + s_[ct][t][1]) + (s_[ct][t][2] + s_[ct][t][3]);
-        if constexpr (Q8) {
+        if constexpr (Q8) {                // (the scale of what is seen counts, also with a weight of 0: it may be NaN)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s_[ct][t][i] = (full || s_[ct][t][i] != 0.f) ? s_[ct][t][i] * vsc[t][i] : 0.f;
+          for (int i = 0; i < 4; ++i) s_[ct][t][i] = (full || (vis[ct] >> (4 * t + i) & 1)) ? s_[ct][t][i] * vsc[t][i] : 0.f;
         }
       }
     }

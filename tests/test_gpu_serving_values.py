@@ -58,3 +58,12 @@ def test_values_without_weight_show_across_waves_and_splits(K, dtype, value, n, 
     """token `bad` lies in a block that is seen whole, in another wave or workgroup than the token that takes all the weight"""
     for Nq, nh, H, D in ((1, 2, 2, 64), (1, 8, 2, 128), (3, 12, 2, 64)):
         _check(_with_and_without(K, dtype, n, Nq, nh, H, D, 32, top, bad, value), dtype, n, Nq, nh, H, bad)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32, I8, E4M3])
+@pytest.mark.parametrize('value', [float('inf'), float('nan')])
+@pytest.mark.parametrize('n,top,bad', [(200, 5, 196), (200, 197, 193), (190, 40, 188), (9001, 4, 8995), (33, 1, 32), (20, 3, 11)])
+def test_values_without_weight_show_in_blocks_seen_in_part(K, dtype, value, n, top, bad):
+    """token `bad` lies in the last, incomplete block (of some, only the later rows see it)"""
+    for Nq, nh, H, D in ((1, 2, 2, 64), (1, 8, 2, 128), (3, 12, 2, 64), (3, 16, 2, 128)):
+        _check(_with_and_without(K, dtype, n, Nq, nh, H, D, 32, top, bad, value), dtype, n, Nq, nh, H, bad)
