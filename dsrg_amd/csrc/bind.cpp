@@ -7,6 +7,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <algorithm>
 #include <climits>
 #include <cstdarg>
 #include <stdexcept>
@@ -296,8 +297,11 @@ PyObject* sample_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (t.scalar_type() != (i == 1 ? at::kInt : at::kFloat) || t.dim() != 1 || t.size(0) != B || !t.is_contiguous() || t.device() != dev)
           refuse("sample_rows: %s must be a number or contiguous %s [B] beside the logits", names[i], i == 1 ? "int32" : "fp32");
         p[i] = B ? t.data_ptr() : nullptr;
-      } else if (i == 1) k0 = as_int(what, names[i], o);
-      else num[i] = as_double(o);
+      } else if (i == 1) k0 = std::max(as_int(what, names[i], o), 0);          // (below 0 is "off" here, or the largest entry, as 0 is in the C-ABI)
+      else {
+        num[i] = as_double(o);
+        if (i != 2 && num[i] < 0) num[i] = 0;
+      }
     }
     const c10::DeviceGuard guard(dev);
     const auto opt = at::TensorOptions().device(dev);

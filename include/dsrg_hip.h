@@ -365,8 +365,10 @@ int dsrg_action_tail_fwd(const float* logits, int ld, const int64_t* targets, in
  * (equal values: the lowest index first) are cut (1) after the k-th (k <= 0: no cut); (2) after the first whose running sum of
  * weights w = exp((x - max) / T) reaches p of the sum over what (1) left (p >= 1: no cut; the first one always stays); (3) before
  * the first with w < m (m <= 0: no cut; m > 1: as 1).  token[b] = the first entry, in index order, at which the running sum over what is left
- * exceeds u[b] times the whole; logp[b] = its log-probability among them.  T <= 0 (or NaN): the largest entry, logp 0.  A row without
- * a candidate: token -1, logp -inf.  1 <= V <= 524288.  Deterministic: sums are 64-bit integers. */
+ * exceeds u[b] times the whole; logp[b] = its log-probability among them.  T <= 0 (or NaN): the largest entry, logp 0; T = inf: all weigh
+ * the same.  NaN among p or m: no cut; p <= 0: the first one.  Numbers instead of arrays are checked: 0 <= T < inf, k >= 0, p >= 0,
+ * 0 <= m <= 1, anything else is DSRG_EINVAL.  A row without a candidate: token -1, logp -inf.  1 <= V <= 524288.  Deterministic: sums
+ * are 64-bit integers. */
 int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature, float temperature0,
                      const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
                      int64_t* token, float* logp, int B, int V, void* stream);
