@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
 #include <climits>
@@ -53,6 +54,12 @@ void on_device(const char* what, const at::Tensor& t) {
   if (!t.is_cuda()) refuse("dsrg_amd kernels need device tensors (%s got %s); there is no CPU path", what, t.device().str().c_str());
 }
 
+// These operators have no backward: what asks for a gradient is refused, since its gradient would be lost without a word
+void no_grad(const char* what, const char* name, const at::Tensor& t) {
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    refuse("%s has no backward and %s asks for a gradient: detach it, or call under torch.no_grad()", what, name);
+}
+
 int io_dtype(const char* what, at::ScalarType t) {
   if (t == at::kFloat) return DSRG_F32;
   if (t == at::kBFloat16) return DSRG_BF16;
@@ -84,6 +91,8 @@ struct Cache { dsrg_kv_cache_t c; int H, D; at::Device dev; };
 
 Cache cache_of(const char* what, PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso) {
   const at::Tensor &k = tensor(what, "k_pool", ko), &v = tensor(what, "v_pool", vo);
+  no_grad(what, "k_pool", k);
+  no_grad(what, "v_pool", v);
   on_device(what, k);
   const at::ScalarType st = k.scalar_type();
   const int dt = st == at::kBFloat16 ? DSRG_BF16 : st == at::kFloat ? DSRG_F32 : st == at::kChar ? DSRG_I8 : st == at::kFloat8_e4m3fn ? DSRG_E4M3 : -1;
@@ -100,6 +109,7 @@ Cache cache_of(const char* what, PyObject* ko, PyObject* vo, PyObject* kso, PyOb
       const bool given = so[i] != Py_None;
       if (given) {
         const at::Tensor& s = tensor(what, "scale", so[i]);
+        no_grad(what, i ? "v_scale" : "k_scale", s);
         if (s.scalar_type() == at::kFloat && s.sizes() == at::IntArrayRef({P, H, S}) && s.is_contiguous() && s.device() == k.device()) { scale[i] = s.data_ptr<float>(); continue; }
       }
       refuse("%s: an 8-bit cache needs k_scale and v_scale, contiguous fp32 [pages, kv heads, page size]", what);
@@ -191,8 +201,10 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const char* what = "kv_append";
     arity(what, n, 9);
-    const Cache c = cache_of(what, a[2], a[3], a[7], a[8]);
     const at::Tensor &k = tensor(what, "k", a[0]), &v = tensor(what, "v", a[1]);
+    no_grad(what, "k", k);
+    no_grad(what, "v", v);
+    const Cache c = cache_of(what, a[2], a[3], a[7], a[8]);
     const int64_t W = (int64_t)c.H * c.D;
     if (k.dim() != 3 || k.size(2) != W || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || k.device() != c.dev || v.device() != c.dev)
       refuse("kv_append: k and v must be [B, T, %lld] of one dtype beside the cache (got %s, %s)", (long long)W, shape_of(k).c_str(), shape_of(v).c_str());
@@ -242,8 +254,9 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const char* what = "attention_paged";
     arity(what, n, 12);
-    const Cache c = cache_of(what, a[1], a[2], a[6], a[7]);
     const at::Tensor& q = tensor(what, "q", a[0]);
+    no_grad(what, "q", q);
+    const Cache c = cache_of(what, a[1], a[2], a[6], a[7]);
     const int nh = as_int(what, "nh", a[5]);
     if (q.dim() != 3 || nh < 1 || nh % c.H || q.size(2) != (int64_t)nh * c.D || q.device() != c.dev)
       refuse("attention_paged: q %s is not [B, Nq, nh * %d] with nh = %d a multiple of %d, beside the cache", shape_of(q).c_str(), c.D, nh, c.H);
@@ -278,13 +291,17 @@ PyObject* sample_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const char* what = "sample_rows";
     arity(what, n, 6);
+    static const char* const names[4] = {"temperature", "top_k", "top_p", "min_p"};
     const at::Tensor &x = tensor(what, "logits", a[0]), &u = tensor(what, "u", a[1]);
+    no_grad(what, "logits", x);
+    no_grad(what, "u", u);
+    for (int i = 0; i < 4; ++i)
+      if (THPVariable_Check(a[2 + i])) no_grad(what, names[i], THPVariable_Unpack(a[2 + i]));
     on_device(what, x);
     if (x.dim() != 2 || x.size(1) < 1 || (x.stride(1) != 1 && x.size(1) > 1)) refuse("sample_rows: logits must be [B,V] with contiguous rows (got %s)", shape_of(x).c_str());
     const int dt = io_dtype(what, x.scalar_type()), B = fits(what, x.size(0)), V = fits(what, x.size(1));
     const at::Device dev = x.device();
     if (u.scalar_type() != at::kFloat || u.dim() != 1 || u.size(0) != B || !u.is_contiguous() || u.device() != dev) refuse("sample_rows: u must be contiguous fp32 [B] beside the logits");
-    static const char* const names[4] = {"temperature", "top_k", "top_p", "min_p"};
     const void* p[4];
     double num[4];
     int k0 = 0;

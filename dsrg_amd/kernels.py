@@ -816,6 +816,7 @@ def action_tail(logits, targets=None, u=None, ignore_index=-100, want_grad=False
 
 
 # ---- serving operators: the checks and the call are native code (csrc/bind.cpp) ----------------------------------------------
+# None has a backward: an input that asks for a gradient while gradients are recorded is refused.
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One entry of each row of logits [B,V] (fp32 / bf16, rows contiguous, -inf and NaN = not a candidate), drawn with the given

@@ -59,6 +59,4 @@ class PagedKVCache:
 
     def attend(self, q, table, lens, nh, scale=None, causal=False, window=0, want_lse=False):
         """kernels.attention_paged over this cache (inference: no gradient)"""
-        if torch.is_grad_enabled() and q.requires_grad:
-            raise DsrgHipError('kv cache: attention over a paged cache has no backward; call it under torch.no_grad()')
         return K.attention_paged(q, self.k_pool, self.v_pool, table, lens, nh, self.k_scale, self.v_scale, scale, causal, window, want_lse)

@@ -127,3 +127,22 @@ def test_no_cpu_path():
             call()
     with pytest.raises(DsrgHipError, match='no backward'):
         c.attend(x.requires_grad_(), t, i, 1)
+
+
+def test_inputs_that_ask_for_a_gradient():
+    """no serving operator has a backward: such an input is refused (before any other look at it), not detached; under no_grad it is one like any other"""
+    ks, vs = K.kv_pool_shapes(2, 32, 1, 64, torch.bfloat16)
+    kp, vp = torch.zeros(ks, dtype=torch.bfloat16), torch.zeros(vs, dtype=torch.bfloat16)
+    x, i, t = torch.zeros(1, 1, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    r, one = x.clone().requires_grad_(), torch.ones(1)
+    grad = lambda y: y.clone().requires_grad_()          # noqa: E731
+    calls = [('k', lambda: K.kv_append(r, x, kp, vp, t, i)), ('v', lambda: K.kv_append(x, r, kp, vp, t, i)), ('q', lambda: K.attention_paged(r, kp, vp, t, i, 1)),
+             ('k_pool', lambda: K.attention_paged(x, grad(kp), vp, t, i, 1)), ('v_pool', lambda: K.kv_read(kp, grad(vp), t, i, i, 1)),
+             ('logits', lambda: K.sample_rows(grad(torch.zeros(1, 4)), one)), ('temperature', lambda: K.sample_rows(torch.zeros(1, 4), one, grad(one))),
+             ('top_p', lambda: K.sample_rows(torch.zeros(1, 4), one, top_p=grad(one))), ('min_p', lambda: K.sample_rows(torch.zeros(1, 4), one, min_p=grad(one)))]
+    for name, call in calls:
+        with pytest.raises(DsrgHipError, match='no backward and %s asks' % name):
+            call()
+        if not torch.cuda.is_available():
+            with torch.no_grad(), pytest.raises(DsrgHipError, match='device tensors'):
+                call()
