@@ -743,7 +743,7 @@ int check_cache(const dsrg_kv_cache_t* c, const char* who, Pool& p) {
   DSRG_CHECK(c && c->k_pool && c->v_pool, "%s: cache pools are NULL", who);
   DSRG_CHECK(c->dtype == DSRG_F32 || c->dtype == DSRG_BF16 || c->dtype == DSRG_I8 || c->dtype == DSRG_E4M3, "%s: unknown cache dtype %d", who, c->dtype);
   DSRG_CHECK(c->head_dim == 64 || c->head_dim == 128, "%s: head dim %d is not built (64, 128)", who, c->head_dim);
-  DSRG_CHECK(c->page_size >= 32 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0, "%s: page size %d must be a power of two from 32 on", who, c->page_size);
+  DSRG_CHECK(c->page_size >= 32 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0, "%s: page size %d must be a power of two from 32 to 65536", who, c->page_size);
   DSRG_CHECK(c->n_pages >= 1 && c->n_kv_heads >= 1, "%s: a cache needs pages and heads (%d, %d)", who, c->n_pages, c->n_kv_heads);
   const bool q8 = c->dtype == DSRG_I8 || c->dtype == DSRG_E4M3;
   DSRG_CHECK(q8 == (c->k_scale != nullptr) && q8 == (c->v_scale != nullptr), "%s: 8-bit caches need both scale tables, the others none", who);

@@ -834,8 +834,8 @@ def kv_pool_shapes(n_pages, page_size, n_kv_heads, head_dim, dtype):
     """(shape of k_pool, shape of v_pool) of a paged cache (dsrg_kv_cache_t)"""
     if dtype not in _KV_DT:
         raise _lib.DsrgHipError('kv cache: unsupported dtype %s (float32 / bfloat16 / int8 / float8_e4m3fn)' % (dtype,))
-    if head_dim not in (64, 128) or page_size < 32 or page_size & (page_size - 1) or n_pages < 1 or n_kv_heads < 1:
-        raise _lib.DsrgHipError('kv cache: head dim 64 or 128, pages of a power of two tokens from 32 on (got head dim %d, %d pages of %d tokens, %d heads)'
+    if head_dim not in (64, 128) or not 32 <= page_size <= 65536 or page_size & (page_size - 1) or n_pages < 1 or n_kv_heads < 1:
+        raise _lib.DsrgHipError('kv cache: head dim 64 or 128, pages of a power of two tokens from 32 to 65536 (got head dim %d, %d pages of %d tokens, %d heads)'
                                 % (head_dim, n_pages, page_size, n_kv_heads))
     if dtype == torch.float32:
         return (n_pages, n_kv_heads, page_size // 16, head_dim // 4, 16, 4), (n_pages, n_kv_heads, page_size // 16, head_dim // 16, 4, 16, 4)

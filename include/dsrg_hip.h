@@ -374,7 +374,7 @@ int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, 
                      int64_t* token, float* logp, int B, int V, void* stream);
 
 /* ---- paged key / value cache (no counterpart in the reference, which keeps padded dense tensors) --------------------
- * Pages of `page_size` tokens (a power of two, 32 or more) hold the keys and values of all heads; token t of sequence b lies in
+ * Pages of `page_size` tokens (a power of two from 32 to 65536) hold the keys and values of all heads; token t of sequence b lies in
  * page table[b * table_ld + t / page_size], row t % page_size; a table has `width` entries a sequence (reaching 2^30 tokens at most).  Inside (page, head):
  *   bf16 and 8 bits:  K [S/16][D/8][16 tokens][8 dims]; V [S/32][D/16][4 g][16 dims][2 m][4 i], token 32 t + 16 m + 4 g + i;
  *   fp32:             K [S/16][D/4][16 tokens][4 dims]; V [S/16][D/16][4 g][16 dims][4 i],      token 16 t + 4 g + i;

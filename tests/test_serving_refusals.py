@@ -146,3 +146,14 @@ def test_inputs_that_ask_for_a_gradient():
         if not torch.cuda.is_available():
             with torch.no_grad(), pytest.raises(DsrgHipError, match='device tensors'):
                 call()
+
+
+def test_pages_too_large_are_refused_where_the_pools_are_made():
+    """the kernels take pages of up to 65536 tokens: a larger cache could be made and then not used"""
+    from dsrg_amd.kvcache import PagedKVCache
+    assert _lib.load().dsrg_attention_paged_workspace(_cache(page_size=1 << 16), 4, 1, 2, 1, 0) >= 0
+    assert _lib.load().dsrg_attention_paged_workspace(_cache(page_size=1 << 17), 4, 1, 2, 1, 0) == -1 and b'65536' in _lib.load().dsrg_last_error()
+    assert K.kv_pool_shapes(1, 1 << 16, 1, 64, torch.int8)[0] == (1, 1, 4096, 8, 16, 8)
+    for f in (lambda: K.kv_pool_shapes(1, 1 << 17, 1, 64, torch.int8), lambda: PagedKVCache(1, 1, 64, device='cpu', dtype=torch.int8, page_size=1 << 17)):
+        with pytest.raises(DsrgHipError, match='65536'):
+            f()
