@@ -313,7 +313,7 @@ struct PagedArgs {
   int q_rs, o_rs;
   const int32_t *table, *lens;
   int table_ld, width, B, nh, G, Nq, NC;       // NC = Nq * G columns per (sequence, key / value head)
-  int causal, window, nsplit, bps;             // bps: 32-token blocks per split
+  int window, nsplit, bps;                     // bps: 32-token blocks per split
   float sl2;                                   // scale * log2(e)
   float* ws_o; float2* ws_ml;                  // [B, H, NC, nsplit, D], [B, H, NC, nsplit]
 };
@@ -906,7 +906,7 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const Split s = plan_split(cache->dtype, D_, ct, B, a.c.H, cgs, seen_tokens(width, a.c.S, Nq, window));
   a.q = q; a.o = o; a.lse = lse; a.q_bs = q_bs; a.o_bs = o_bs; a.q_rs = q_rs; a.o_rs = o_rs;
   a.table = table; a.lens = lens; a.table_ld = table_ld; a.width = width; a.B = B; a.nh = nh; a.Nq = Nq;
-  a.causal = causal != 0; a.window = window < (long long)width * a.c.S ? window : 0; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
+  a.window = window < (long long)width * a.c.S ? window : 0; a.nsplit = s.nsplit; a.bps = s.bps; a.sl2 = scale * LOG2E;
   a.ws_o = (float*)workspace;
   a.ws_ml = need ? (float2*)((float*)workspace + (int64_t)B * a.c.H * a.NC * s.nsplit * D_) : nullptr;
   const long long rows = (long long)B * a.c.H * a.NC;
