@@ -448,8 +448,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const SampleArgs a) {
     for (int i = tid; i < n; i += NT) {                 // what is not kept loses its weight: it is not drawn then
       const ulonglong2 me = list[i];
       const float x = value(me.x);
-      const unsigned rank = cuts ? l_rank[i] : 1u;      // (the first one stays, as min-p keeps its equals)
-      const bool keep = rank == 0 || (rank < want && (!(p < 1.f) || (double)l_ahead[i] < goal) && (x == mx || (double)x >= floor_));
+      // (without cuts all entries are among the first `want`, and the largest stays by min-p)
+      const unsigned rank = cuts ? l_rank[i] : 0u;
+      const bool first = cuts && rank == 0, in = rank < want && (!(p < 1.f) || (double)l_ahead[i] < goal);
+      const bool keep = first || (in && (x == mx || (double)x >= floor_));
       if (keep) sum += me.y; else list[i].y = 0;
     }
     sum = wave_sum_u64(sum);
