@@ -118,7 +118,7 @@ struct AppendArgs {
 };
 
 // D / 8 lanes per (sequence, token, head) row, 8 dims each, K and V of the row by the same lanes.  For few tokens of a sequence: bound by
-// the launch (64 tokens of 12 heads of 64: 4.1 us), V's scattered elements do not show.
+// the launch (64 tokens of 12 heads of 64: 4.2 us), V's scattered elements do not show.
 template <int KV, int D, typename TI>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   typedef typename KvT<KV>::type TS;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
 // by a second kernel.
 // Bound by HBM where there is enough to read: 32 sequences of 1000-32768 tokens, 64 / 8 heads of 128, bf16: 2.21 GB in 430 us (5.15 TB/s; a 4 GiB
 // copy moves 4.75); 3 of 40-60 thousand in e4m3: 317 MB in 65 us with the join.  64 of 1-2011 tokens, 12 heads of 64, int8: 105 MB in
-// 28 us, the longest first.  One of 200 tokens: 4.3 us, the chain launch - length - page - keys - output.
+// 28 us, the longest first.  One of 200 tokens: 4.5 us, the chain launch - length - page - keys - output.
 struct PagedArgs {
   Pool c;
   const void* q; void* o; float* lse;
@@ -346,13 +346,13 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(u32x2 u, int kv) {
   return r;
 }
 
-// MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
 // Waves that a SIMD holds: bounded by the registers of O, of the step's keys and values and of the queries.
 constexpr int resident(int kv, int D, int CT) {
   return D == 64 ? (CT == 1 ? 4 : 3) - (kv == DSRG_F32) : kv == DSRG_F32 ? 1 : kv != DSRG_BF16 && CT == 1 ? 3 : 2;
 }
 // Waves of a large workgroup (one column tile): all that a CU holds, so that a sequence's tokens are joined in LDS as far as that goes
 constexpr int most_waves(int kv, int D, int CT) { return CT > 1 ? 4 : 4 * resident(kv, D, 1); }
+// MIX: the columns see different tokens (causal with several rows); otherwise all see [lo, len) and no per-column bounds are kept.
 template <int KV, int D, int CT, int NW, bool MIX, bool LF>
 __global__ __launch_bounds__(NW * 64, resident(KV, D, CT)) void attention_paged_kernel(const PagedArgs a) {
   typedef typename KvT<KV>::type TS;
@@ -767,6 +767,9 @@ struct Split { int nw, nsplit, bps; };
 // more): large workgroups where four waves are not enough, and splits only where one of them is not.  (26 thousand tokens of one sequence, two
 // heads of 128: 51 workgroups of 8 waves 14.3 us, 102 of 4 17.4; 16 sequences of up to 999, 12 fp32 heads: one of 12 waves each 17.2 us, 5 of 4
 // waves and the join 18.6; 264 workgroups instead of 240 on 256 CUs: 101 us instead of 66 for three sequences of 60 thousand.)
+// The tokens are those that the table reaches, since the host knows no lengths: a table much wider than its sequences costs a join and
+// leaves waves without work (one of 200 tokens, 12 heads of 64: 4.7 us, in a table of 8192 8.8; 8 of 1000, 8 heads of 128: 10.6 and 20.1; 64 of
+// 1-2011 int8 tokens: 24.2, in a table of 32768 44.2).
 Split plan_split(int kv, int D, int ct, int B, int H, int cgs, long long max_tokens) {
   const long long blocks = std::max((max_tokens + 31) / 32, 1ll), have = (long long)B * H * cgs, places = 1024ll * resident(kv, D, ct), most = most_waves(kv, D, ct);
   const long long waves = std::max(std::min(places / have, (blocks + 1) / 2), 4ll);
@@ -914,7 +917,8 @@ extern "C" int dsrg_attention_paged(const dsrg_kv_cache_t* cache, const void* q,
   const dim3 grid(s.nsplit, a.c.H * cgs, B);
   const hipStream_t st = (hipStream_t)stream;
   const bool mix = causal && Nq > 1;
-  // longest sequences first (in an instantiation of its own: it costs other calls 1 to 4 %): long sequences, several workgroups of four waves a CU
+  // longest sequences first (in an instantiation of its own: it costs other calls 1 to 4 %): long sequences, several workgroups of four waves a CU.
+  // One lane ranks a sequence, so 64 at most (of 1-2011 int8 tokens: 64 sequences in this order 24.2 us, 65 in theirs 29.1).
   const bool lf = s.nsplit == 1 && s.nw == 4 && B > 1 && B <= 64 && a.c.H * cgs * B > 256 && !a.window && (long long)width * a.c.S >= 1024;
   KV_SWITCH(cache->dtype, D_SWITCH(D_, {
     constexpr int MW = most_waves(KV, D, 1);

@@ -5,11 +5,13 @@
 // falls under m times the largest.  So nothing is sorted: a cut is a threshold on the 64-bit number (value's order-preserving
 // bits, ~index), found from a histogram (count or weight per bin of max - x) and the exact ranks inside the one bin that the cut
 // falls into.  The draw is the inverse distribution function over what is left, in index order.
-// Weights exp((x - max) / T) are fixed-point numbers of 44 bits behind the point (relative error below 1e-10): integer sums do not
-// depend on the order of the atomics, and 2^-45 an entry is far below what a 24-bit random number resolves.
-// One workgroup a row.  Measured (fp32): 256 rows of 30522, k = 60, p = 0.92, m = 0.02: 14 us, of which the 31 MB take 5.3 (5.9 TB/s) and the
-// rest is one workgroup's chain of barriers; 64 rows of 100 with top-p: 5.4 us, the launch and the same chain; 64 rows of 30522 with
-// top-p alone 36 us and unfiltered 17 us, bound by the weights' instructions (one or two weights an entry, 29 instructions each) on 64 CUs.
+// Weights exp((x - max) / T) are fixed-point numbers with 44 bits behind the point, good to 1e-10 of themselves and cut off at 2^-44 of the
+// largest (lighter entries weigh nothing): integer sums do not depend on the order of the atomics, and 2^-44 an entry is at most 2^-25 of
+// the largest weight a row, half a step of a 24-bit random number.
+// One workgroup a row.  Measured (fp32): 256 rows of 30522, k = 60, p = 0.92, m = 0.02: 14.1 us, of which the 31 MB take 5.3 (5.9 TB/s) and the
+// rest is one workgroup's chain of barriers; 64 rows of 100 with top-p: 5.5 us, the launch and the same chain; 64 rows of 30522 with
+// top-p alone (0.9) 33 us and unfiltered 16.5 us, bound by the weights' instructions (one or two weights an entry, 29 instructions each) on 64
+// CUs; rows of 131072, read again by every pass: 55 us unfiltered and 124 us with top-p for one row, 58 and 129 for 64.
 #include "common.h"
 #include <math.h>
 

@@ -819,7 +819,7 @@ def action_tail(logits, targets=None, u=None, ignore_index=-100, want_grad=False
 # None has a backward: an input that asks for a gradient while gradients are recorded is refused.
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """One entry of each row of logits [B,V] (fp32 / bf16, rows contiguous, -inf and NaN = not a candidate), drawn with the given
+    """One entry of each row of logits [B,V] (fp32 / bf16, rows contiguous and apart, -inf and NaN = not a candidate), drawn with the given
     numbers u fp32 [B] in [0, 1): -> (token int64 [B], logp fp32 [B]).  temperature (<= 0: the largest entry), top_k (<= 0: off), top_p (>= 1: off)
     and min_p (<= 0: off) are numbers or tensors [B] (fp32, top_k int32); NaN, a temperature of infinity, a top_p below 0 and a min_p over 1 are
     refused as numbers, what a tensor's do says dsrg_sample_rows.  The cuts apply in that order, each to what the one before left; equal

@@ -43,7 +43,8 @@ class PagedKVCache:
         return rows.to(self.k_pool.device)
 
     def release(self, table):
-        """Gives a table's pages back (copies the table to the host)"""
+        """Gives a table's pages back (copies the table to the host).  A page that several sequences share is given back once: put -1 in its
+        place in the others' tables."""
         pages = [p for p in table.reshape(-1).tolist() if p >= 0]
         if len(set(pages)) < len(pages) or any(p >= self.n_pages for p in pages) or set(pages) & set(self._free):
             raise DsrgHipError('kv cache: these pages are not taken')

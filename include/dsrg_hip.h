@@ -367,8 +367,9 @@ int dsrg_action_tail_fwd(const float* logits, int ld, const int64_t* targets, in
  * the first with w < m (m <= 0: no cut; m > 1: as 1).  token[b] = the first entry, in index order, at which the running sum over what is left
  * exceeds u[b] times the whole; logp[b] = its log-probability among them.  T <= 0 (or NaN): the largest entry, logp 0; T = inf: all weigh
  * the same.  NaN among p or m: no cut; p <= 0: the first one.  Numbers instead of arrays are checked: 0 <= T < inf, k >= 0, p >= 0,
- * 0 <= m <= 1, anything else is DSRG_EINVAL.  A row without a candidate: token -1, logp -inf.  1 <= V <= 524288.  Deterministic: sums
- * are 64-bit integers. */
+ * 0 <= m <= 1, anything else is DSRG_EINVAL.  A row without a candidate: token -1, logp -inf.  1 <= V <= 524288, ld >= V for several rows.
+ * Deterministic: sums are 64-bit integers of weights cut off at 2^-44 of the largest (a lighter candidate is never drawn, nor does it move
+ * the cut at p). */
 int dsrg_sample_rows(const void* logits, int64_t ld, int dtype, const float* u, const float* temperature, float temperature0,
                      const int32_t* top_k, int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
                      int64_t* token, float* logp, int B, int V, void* stream);
